@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -29,8 +30,16 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xptxas", "-v",
-    "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
+    "-Xcompiler", "-fPIC,-fvisibility=hidden",
 ]
+
+# The translation units of libkvmig.so, with the headers each includes besides the common ones.
+KVMIG_SOURCES = {
+    "kvmig": ["kvmig_kernels.cuh"],
+    "kvcache": ["kvcache_device.cuh"],
+    "kvattn": ["kvcache_device.cuh"],
+}
+SHIM_SOURCES = ["st_pybinding.cpp", "cache_ops.cpp"]
 
 
 def _nvcc() -> str:
@@ -55,11 +64,20 @@ def _run(cmd, log_name: str) -> None:
 
 
 def build_kvmig(force: bool = False) -> Path:
-    src = CSRC / "kvmig.cu"
     hdr = INCLUDE / "kvmig.h"
+    headers = [hdr, CSRC / "kvmig_common.h"]
     LIB.mkdir(exist_ok=True)
-    if force or _stale(KVMIG_SO, [src, hdr, CSRC / "kvmig_kernels.cuh"]):
-        _run([_nvcc(), *NVCC_FLAGS, "-o", KVMIG_SO, src], "libkvmig.build.log")
+    objects, jobs = [], []
+    for name, own_headers in KVMIG_SOURCES.items():
+        src, obj = CSRC / f"{name}.cu", LIB / f"{name}.o"
+        objects.append(obj)
+        if force or _stale(obj, [src, *headers, *(CSRC / h for h in own_headers)]):
+            jobs.append(([_nvcc(), *NVCC_FLAGS, "-c", "-o", obj, src], f"{name}.build.log"))
+    with ThreadPoolExecutor(max_workers=max(1, len(jobs))) as pool:
+        for done in [pool.submit(_run, *job) for job in jobs]:
+            done.result()
+    if force or _stale(KVMIG_SO, objects):
+        _run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", KVMIG_SO, *objects], "libkvmig.build.log")
     return KVMIG_SO
 
 
@@ -67,17 +85,17 @@ def build_shim(force: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    src = CSRC / "st_pybinding.cpp"
+    sources = [CSRC / name for name in SHIM_SOURCES]
     hdr = INCLUDE / "kvmig.h"
     LIB.mkdir(exist_ok=True)
-    if force or _stale(SHIM_SO, [src, hdr, KVMIG_SO]):
+    if force or _stale(SHIM_SO, [*sources, hdr, KVMIG_SO]):
         torch_lib = Path(torch.__file__).resolve().parent / "lib"
         cuda_home = Path(_nvcc()).resolve().parent.parent
         cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
         for inc in cpp_extension.include_paths():
             cmd += ["-isystem", inc]
-        cmd += ["-isystem", cuda_home / "include", "-o", SHIM_SO, src,
+        cmd += ["-isystem", cuda_home / "include", "-o", SHIM_SO, *sources,
                 f"-L{LIB}", "-lkvmig", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
                 "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}", "-Wl,--no-as-needed"]
         _run(cmd, "libst_pybinding.build.log")

@@ -29,6 +29,23 @@ class PoolShape(C.Structure):
         return self.num_layers * self.num_heads * self.block_size * self.head_dim * self.elem_size
 
 
+F16, BF16 = 0, 1                 # the 16-bit type of rows outside the cache, and of pools that hold 16-bit values
+SCALE_BYTES = 4                  # per row, carried by the last dimension of a quantised pool
+
+
+class Rows(C.Structure):
+    """Rows of tokens outside the cache, [num_rows, num_heads, head_dim]; strides in elements."""
+
+    _fields_ = [("data", C.c_void_p), ("num_heads", C.c_int64), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Batch(C.Structure):
+    """The sequences of a batch; the three arrays are int32 in device memory (or 0 where a call does not use them)."""
+
+    _fields_ = [("num_seqs", C.c_int64), ("num_rows", C.c_int64), ("max_rows", C.c_int64), ("starts", C.c_void_p),
+                ("seq_lens", C.c_void_p), ("block_tables", C.c_void_p), ("table_stride", C.c_int64), ("max_blocks", C.c_int64)]
+
+
 class KvmigError(RuntimeError):
     def __init__(self, code: int, text: str):
         super().__init__(f"{text} (kvmig status {code})")
@@ -37,6 +54,8 @@ class KvmigError(RuntimeError):
 
 _I64P = C.POINTER(C.c_int64)
 _SHAPEP = C.POINTER(PoolShape)
+_ROWSP = C.POINTER(Rows)
+_BATCHP = C.POINTER(Batch)
 
 # name -> (restype, argtypes); one entry per declaration in include/kvmig.h
 SIGNATURES = {
@@ -58,6 +77,12 @@ SIGNATURES = {
                                               C.c_int64, _I64P, C.c_int64, C.c_void_p, C.c_void_p, _SHAPEP, C.c_void_p]),
     "kvmig_swap": (C.c_int, [_I64P, C.c_int64, _I64P, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, _SHAPEP, C.c_void_p,
                              C.c_void_p, C.c_int64, C.c_void_p]),
+    "kvmig_cache_write": (C.c_int, [_ROWSP, _ROWSP, C.c_int, C.c_void_p, C.c_void_p, _SHAPEP, C.c_int64, _BATCHP, C.c_void_p]),
+    "kvmig_cache_read": (C.c_int, [C.c_void_p, C.c_void_p, _SHAPEP, C.c_int64, _BATCHP, _ROWSP, _ROWSP, C.c_int, C.c_void_p]),
+    "kvmig_paged_attention_workspace": (C.c_int64, [_SHAPEP, C.c_int64, _BATCHP]),
+    "kvmig_paged_attention": (C.c_int, [_ROWSP, _ROWSP, C.c_int, C.c_void_p, C.c_void_p, _SHAPEP, C.c_int64, _BATCHP, C.c_double,
+                                        C.c_void_p, C.c_int64, C.c_void_p]),
+    "kvmig_prompt_attention": (C.c_int, [_ROWSP, _ROWSP, _ROWSP, _ROWSP, C.c_int, C.c_int64, _BATCHP, C.c_double, C.c_void_p]),
     "kvmig_set_option": (C.c_int, [C.c_char_p, C.c_int64]),
     "kvmig_get_option": (C.c_int64, [C.c_char_p]),
     "kvmig_get_counter": (C.c_int64, [C.c_char_p]),
@@ -174,6 +199,36 @@ def swap(source_ids, target_ids, is_swap_in: bool, k_ptr, v_ptr, shape: PoolShap
          num_cpu_blocks: int, stream: int = 0) -> None:
     _check(lib().kvmig_swap(_i64(source_ids), len(source_ids), _i64(target_ids), len(target_ids), int(bool(is_swap_in)),
                             k_ptr, v_ptr, C.byref(shape), k_swap_ptr, v_swap_ptr, num_cpu_blocks, stream))
+
+
+def cache_write(k: Rows, v: Rows, dtype: int, k_ptr: int, v_ptr: int, shape: PoolShape, layer: int, batch: Batch, stream: int = 0) -> None:
+    """Put the batch's new tokens into one layer of the pools; enqueued on `stream`."""
+    _check(lib().kvmig_cache_write(C.byref(k), C.byref(v), dtype, k_ptr, v_ptr, C.byref(shape), layer, C.byref(batch), stream))
+
+
+def cache_read(k_ptr: int, v_ptr: int, shape: PoolShape, layer: int, batch: Batch, k_out: Rows, v_out: Rows, dtype: int, stream: int = 0) -> None:
+    """Read the batch's sequences from one layer of the pools; enqueued on `stream`."""
+    _check(lib().kvmig_cache_read(k_ptr, v_ptr, C.byref(shape), layer, C.byref(batch), C.byref(k_out), C.byref(v_out), dtype, stream))
+
+
+def paged_attention_workspace(shape: PoolShape, num_q_heads: int, batch: Batch) -> int:
+    """Bytes of device memory that paged_attention needs for these sizes."""
+    n = lib().kvmig_paged_attention_workspace(C.byref(shape), num_q_heads, C.byref(batch))
+    if n < 0:
+        _check(n)
+    return n
+
+
+def paged_attention(q: Rows, out: Rows, dtype: int, k_ptr: int, v_ptr: int, shape: PoolShape, layer: int, batch: Batch, scale: float,
+                    workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+    """Attention of the batch's rows over their sequences' cache; enqueued on `stream`."""
+    _check(lib().kvmig_paged_attention(C.byref(q), C.byref(out), dtype, k_ptr, v_ptr, C.byref(shape), layer, C.byref(batch), scale,
+                                       workspace, workspace_bytes, stream))
+
+
+def prompt_attention(q: Rows, k: Rows, v: Rows, out: Rows, dtype: int, head_dim: int, batch: Batch, scale: float, stream: int = 0) -> None:
+    """Causal attention of whole packed prompts; enqueued on `stream`."""
+    _check(lib().kvmig_prompt_attention(C.byref(q), C.byref(k), C.byref(v), C.byref(out), dtype, head_dim, C.byref(batch), scale, stream))
 
 
 def set_option(name: str, value: int) -> None:

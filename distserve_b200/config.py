@@ -44,10 +44,14 @@ class ParallelConfig:
 
 
 class CacheConfig:
-    """Block size and per-request block cap (distserve/config.py CacheConfig)."""
+    """Block size and per-request block cap (distserve/config.py CacheConfig).  ``kv_format`` says what the pools
+    hold: "model", the model's own type, or "e4m3", one byte per value and a scale per token and head."""
 
     def __init__(self, block_size: int, max_num_blocks_per_req: int,
-                 gpu_memory_utilization: float = 0.9, cpu_swap_space: int = 0) -> None:
+                 gpu_memory_utilization: float = 0.9, cpu_swap_space: int = 0, kv_format: str = "model") -> None:
+        if kv_format not in ("model", "e4m3"):
+            raise ValueError(f"kv_format must be 'model' or 'e4m3', not {kv_format!r}")
+        self.kv_format = kv_format
         self.block_size = block_size
         self.max_num_blocks_per_req = max_num_blocks_per_req
         self.gpu_memory_utilization = gpu_memory_utilization
@@ -102,8 +106,10 @@ class KVModelConfig:
             return 0, 1
         return pc.tensor_parallel_rank * n, (pc.tensor_parallel_rank + 1) * n
 
-    def block_bytes(self, pc: ParallelConfig, block_size: int) -> int:
-        """Bytes of one block of one pool (K or V) on a worker."""
+    def block_bytes(self, pc: ParallelConfig, block_size: int, kv_format: str = "model") -> int:
+        """Bytes of one block of one pool (K or V) on a worker; "e4m3": a byte per value and 4 per row for its scale."""
+        if kv_format == "e4m3":
+            return self.get_num_layers(pc) * self.get_num_heads(pc) * block_size * (self.head_dim + 4)
         return self.get_num_layers(pc) * self.get_num_heads(pc) * block_size * self.head_dim * self.get_dtype_size()
 
 

@@ -1,0 +1,217 @@
+// Causal attention of new tokens over the paged cache, and of whole packed prompts.
+//
+//   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j - m),   m = max_j (scale q . k_j)
+//
+// in one pass over the keys: when the running maximum grows from m to m', what has been summed so far is multiplied
+// by exp(m - m').
+#include "kvcache_device.cuh"
+#include "kvmig_common.h"
+
+#include <cmath>
+
+namespace kvmig {
+namespace {
+
+struct AttnRows {
+    char* data;
+    int64_t row_stride, head_stride;   // bytes
+};
+
+struct AttnParams {
+    AttnRows q, out, k, v;             // k, v: whole prompts only
+    CacheView cache;
+    BatchView batch;
+    int32_t heads, group;              // query heads, query heads per KV head
+    float scale_log2;                  // scale * log2(e): exponentials are taken to base 2
+};
+
+constexpr int kWarps = 4;
+
+// One warp per row and query head, one key at a time.
+template <int HD, bool BF16, bool PAGED, bool E4M3>
+__global__ void __launch_bounds__(kWarps * 32) attend_simple(const __grid_constant__ AttnParams p) {
+    using H = Half<BF16>;
+    constexpr int N = HD / 64;         // pairs of values that a lane holds
+    const int64_t warp = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, head = (int)(warp % p.heads);
+    const int64_t row64 = warp / p.heads;
+    if (row64 >= p.batch.num_rows) return;
+    const int row = (int)row64, i = find_sequence(p.batch.starts, p.batch.num_seqs, row);
+    const Sequence s = sequence_at(p.batch, i);
+    if (!s.valid || row < s.first || row - s.first >= s.rows) return;
+    const int64_t last = PAGED ? (int64_t)p.batch.seq_lens[i] - s.rows + (row - s.first) : row - s.first;
+    float2 q[N], o[N];
+    const char* qp = p.q.data + row * p.q.row_stride + head * p.q.head_stride;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        q[n] = H::to_float2(reinterpret_cast<const uint32_t*>(qp)[lane * N + n]);
+        o[n] = make_float2(0.f, 0.f);
+    }
+    float m = -INFINITY, l = 0.f;
+    bool bad = s.rows > p.batch.max_rows;
+    const int kv_head = head / p.group;
+    for (int64_t j = 0; j <= last && !bad; ++j) {
+        float2 k[N], v[N];
+        if (PAGED) {
+            const int id = j <= INT32_MAX ? block_of(p.batch, p.cache, i, (int)j) : -1;
+            if (id < 0) { bad = true; break; }
+            const int off = (int)(j % p.cache.block_size);
+            const int64_t tile = id * p.cache.block_stride + (int64_t)kv_head * p.cache.head_stride;
+            if (E4M3) {
+                const int64_t at = tile + off * HD + lane * N * 2, sc = tile + p.cache.block_size * HD + off * 4;
+                const float ks = *reinterpret_cast<const float*>(p.cache.k + sc), vs = *reinterpret_cast<const float*>(p.cache.v + sc);
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    k[n] = decode2(reinterpret_cast<const uint16_t*>(p.cache.k + at)[n]);
+                    v[n] = decode2(reinterpret_cast<const uint16_t*>(p.cache.v + at)[n]);
+                    k[n].x *= ks; k[n].y *= ks; v[n].x *= vs; v[n].y *= vs;
+                }
+            } else {
+                const int64_t at = tile + off * HD * 2 + lane * N * 4;
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    k[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.cache.k + at)[n]);
+                    v[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.cache.v + at)[n]);
+                }
+            }
+        } else {
+            const int64_t r = s.first + j;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                k[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.k.data + r * p.k.row_stride + kv_head * p.k.head_stride)[lane * N + n]);
+                v[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.v.data + r * p.v.row_stride + kv_head * p.v.head_stride)[lane * N + n]);
+            }
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) dot += q[n].x * k[n].x + q[n].y * k[n].y;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        dot *= p.scale_log2;
+        const float top = fmaxf(m, dot), keep = exp2f(m - top), e = exp2f(dot - top);
+        m = top;
+        l = l * keep + e;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            o[n].x = o[n].x * keep + e * v[n].x;
+            o[n].y = o[n].y * keep + e * v[n].y;
+        }
+    }
+    const float inv = bad ? __uint_as_float(0x7fffffffu) : l > 0.f ? 1.f / l : 0.f;
+    uint32_t* op = reinterpret_cast<uint32_t*>(p.out.data + row * p.out.row_stride + head * p.out.head_stride);
+#pragma unroll
+    for (int n = 0; n < N; ++n) op[lane * N + n] = H::from_float2(o[n].x * inv, o[n].y * inv);
+}
+
+template <int HD, bool BF16>
+void launch_simple(const AttnParams& p, bool paged, bool e4m3, unsigned grid, cudaStream_t stream) {
+    if (!paged) attend_simple<HD, BF16, false, false><<<grid, kWarps * 32, 0, stream>>>(p);
+    else if (!e4m3) attend_simple<HD, BF16, true, false><<<grid, kWarps * 32, 0, stream>>>(p);
+    else attend_simple<HD, BF16, true, true><<<grid, kWarps * 32, 0, stream>>>(p);
+}
+
+int attend(AttnParams& p, bool paged, bool e4m3, int64_t head_dim, int dtype, const kvmig_batch* batch, cudaStream_t stream, const char* what) {
+    p.batch = BatchView{batch->starts, batch->seq_lens, batch->block_tables, batch->table_stride, (int32_t)batch->num_seqs,
+                        (int32_t)batch->num_rows, (int32_t)batch->max_rows, (int32_t)batch->max_blocks};
+    int dev;
+    CU_TRY(cudaGetDevice(&dev));
+    if (batch->num_rows == 0 || batch->num_seqs == 0) return 0;
+    const int64_t grid = (batch->num_rows * p.heads + kWarps - 1) / kWarps;
+    if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
+    if (head_dim == 64 && dtype == KVMIG_F16) launch_simple<64, false>(p, paged, e4m3, (unsigned)grid, stream);
+    else if (head_dim == 64) launch_simple<64, true>(p, paged, e4m3, (unsigned)grid, stream);
+    else if (dtype == KVMIG_F16) launch_simple<128, false>(p, paged, e4m3, (unsigned)grid, stream);
+    else launch_simple<128, true>(p, paged, e4m3, (unsigned)grid, stream);
+    CU_TRY(cudaGetLastError());
+    g_attention_launches++;
+    return 0;
+}
+
+AttnRows view(const kvmig_rows* r) { return AttnRows{static_cast<char*>(r->data), r->row_stride * 2, r->head_stride * 2}; }
+
+// Checks that the two attention entry points share.
+int check_attention(const kvmig_rows* q, const kvmig_rows* out, int64_t head_dim, int64_t kv_heads, const kvmig_batch* batch,
+                    double scale, const char* what) {
+    if (head_dim != 64 && head_dim != 128) return fail(KVMIG_EINVAL, "%s: head_dim %lld is neither 64 nor 128", what, (long long)head_dim);
+    int rc = check_rows(q, head_dim, batch->num_rows, what);
+    if (!rc) rc = check_rows(out, head_dim, batch->num_rows, what);
+    if (rc) return rc;
+    if (q->num_heads != out->num_heads) return fail(KVMIG_EINVAL, "%s: q has %lld heads, out %lld", what, (long long)q->num_heads, (long long)out->num_heads);
+    if (q->num_heads % kv_heads)
+        return fail(KVMIG_EINVAL, "%s: %lld query heads do not split over %lld KV heads", what, (long long)q->num_heads, (long long)kv_heads);
+    if (!std::isfinite((float)scale * 1.4426950408889634f)) return fail(KVMIG_EINVAL, "%s: scale is not finite", what);
+    return 0;
+}
+
+}  // namespace
+}  // namespace kvmig
+
+using namespace kvmig;
+
+extern "C" {
+
+int64_t kvmig_paged_attention_workspace(const kvmig_pool_shape* shape, int64_t num_q_heads, const kvmig_batch* batch) {
+    clear_error();
+    int rc = check_shape(shape, "paged_attention_workspace");
+    if (!rc) rc = check_batch(batch, false, false, "paged_attention_workspace");
+    if (rc) return rc;
+    if (num_q_heads <= 0 || num_q_heads % shape->num_heads)
+        return fail(KVMIG_EINVAL, "paged_attention_workspace: %lld query heads do not split over %lld KV heads", (long long)num_q_heads,
+                    (long long)shape->num_heads);
+    return 0;
+}
+
+int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype, void* k_cache, void* v_cache,
+                          const kvmig_pool_shape* shape, int64_t layer, const kvmig_batch* batch, double scale, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+    clear_error();
+    const char* what = "paged_attention";
+    int rc = check_pools(k_cache, v_cache, shape, layer, dtype, what);
+    if (!rc) rc = check_batch(batch, true, true, what);
+    if (rc) return rc;
+    const bool e4m3 = shape->elem_size == 1;
+    const int64_t head_dim = shape->head_dim - (e4m3 ? KVMIG_SCALE_BYTES : 0);
+    rc = check_attention(q, out, head_dim, shape->num_heads, batch, scale, what);
+    if (rc) return rc;
+    const int64_t need = kvmig_paged_attention_workspace(shape, q->num_heads, batch);
+    if (need < 0) return (int)need;
+    if (workspace_bytes < need || (need > 0 && (!workspace || (uintptr_t)workspace % 16)))
+        return fail(KVMIG_EINVAL, "%s: needs a workspace of %lld bytes at a multiple of 16", what, (long long)need);
+    AttnParams p = {};
+    p.q = view(q);
+    p.out = view(out);
+    const int64_t tile = shape->block_size * shape->head_dim * shape->elem_size, at_layer = layer * shape->num_heads * tile;
+    p.cache = CacheView{static_cast<char*>(k_cache) + at_layer, static_cast<char*>(v_cache) + at_layer,
+                        shape->num_layers * shape->num_heads * tile, (int32_t)tile, (int32_t)shape->num_blocks,
+                        (int32_t)shape->block_size};
+    p.heads = (int32_t)q->num_heads;
+    p.group = (int32_t)(q->num_heads / shape->num_heads);
+    p.scale_log2 = (float)(scale * 1.4426950408889634);
+    return attend(p, true, e4m3, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
+}
+
+int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig_rows* v, const kvmig_rows* out, int dtype,
+                           int64_t head_dim, const kvmig_batch* batch, double scale, void* stream) {
+    clear_error();
+    const char* what = "prompt_attention";
+    int rc = check_batch(batch, false, false, what);
+    if (rc) return rc;
+    if (dtype != KVMIG_F16 && dtype != KVMIG_BF16) return fail(KVMIG_EINVAL, "%s: unknown dtype %d", what, dtype);
+    if (!(rc = check_rows(k, head_dim, batch->num_rows, what))) rc = check_rows(v, head_dim, batch->num_rows, what);
+    if (rc) return rc;
+    if (k->num_heads != v->num_heads)
+        return fail(KVMIG_EINVAL, "%s: k has %lld heads, v %lld", what, (long long)k->num_heads, (long long)v->num_heads);
+    rc = check_attention(q, out, head_dim, k->num_heads, batch, scale, what);
+    if (rc) return rc;
+    AttnParams p = {};
+    p.q = view(q);
+    p.out = view(out);
+    p.k = view(k);
+    p.v = view(v);
+    p.heads = (int32_t)q->num_heads;
+    p.group = (int32_t)(q->num_heads / k->num_heads);
+    p.scale_log2 = (float)(scale * 1.4426950408889634);
+    return attend(p, false, false, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
+}
+
+}  // extern "C"

@@ -1,0 +1,134 @@
+// Device code shared by the cache kernels (kvcache.cu) and the attention kernels (kvattn.cu): where a token lies in
+// a paged pool, and the conversions between 16-bit rows and e4m3 codes.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace kvmig {
+
+// One layer of a pool pair, and the block tables that lead into it.  Byte addresses: a pool of more than 2^31
+// elements is ordinary, so every product with a block number is 64-bit.
+struct CacheView {
+    char* k;                       // address of (block 0, this layer, head 0)
+    char* v;
+    int64_t block_stride;          // bytes from one block to the next
+    int32_t head_stride;           // bytes from one head's tile to the next
+    int32_t num_blocks, block_size;
+};
+
+struct BatchView {
+    const int32_t* starts;
+    const int32_t* seq_lens;
+    const int32_t* block_tables;
+    int64_t table_stride;
+    int32_t num_seqs, num_rows, max_rows, max_blocks;
+};
+
+// The last sequence that starts at or before row t, found by all lanes of a warp together: each step probes 32
+// places at once, so a batch of up to 32 sequences takes one load and one of up to 1024 two.
+__device__ __forceinline__ int find_sequence(const int32_t* starts, int n, int t) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, count = n;                       // the answer is in [lo, lo + count)
+    while (count > 1) {
+        const int step = (count + 31) / 32;
+        const int at = lo + lane * step;
+        const bool before = at < lo + count && starts[at] <= t;
+        const int hits = __popc(__ballot_sync(0xffffffffu, before));
+        if (hits == 0) return lo;
+        const int next = lo + (hits - 1) * step;
+        count = min(step, lo + count - next);
+        lo = next;
+    }
+    return lo;
+}
+
+struct Sequence {
+    int first, rows;    // its rows
+    bool valid;
+};
+
+__host__ __device__ __forceinline__ Sequence sequence_at(const BatchView& b, int i) {
+    Sequence s;
+    s.first = b.starts[i];
+    const int end = b.starts[i + 1];
+    s.valid = s.first >= 0 && end >= s.first && end <= b.num_rows;
+    s.rows = s.valid ? end - s.first : 0;
+    return s;
+}
+
+// Block that holds position `pos` (>= 0) of a sequence, or -1 if the table or the pool has no such block.
+__host__ __device__ __forceinline__ int block_of(const BatchView& b, const CacheView& c, int seq, int pos) {
+    const int entry = pos / c.block_size;
+    if (entry >= b.max_blocks) return -1;
+    const int id = b.block_tables[seq * b.table_stride + entry];
+    return (unsigned)id < (unsigned)c.num_blocks ? id : -1;
+}
+
+// ---- 16-bit types ----------------------------------------------------------------------------------------
+
+template <bool BF16> struct Half;
+template <> struct Half<false> {
+    using T = __half;
+    using T2 = __half2;
+    static constexpr uint32_t kInf = 0x7c00, kMax = 0x7bff, kNan2 = 0x7fff7fff;
+    static __device__ __forceinline__ float2 to_float2(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+    static __device__ __forceinline__ uint32_t from_float2(float a, float b) {
+        __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float largest() { return 65504.f; }
+};
+template <> struct Half<true> {
+    using T = __nv_bfloat16;
+    using T2 = __nv_bfloat162;
+    static constexpr uint32_t kInf = 0x7f80, kMax = 0x7f7f, kNan2 = 0x7fff7fff;
+    static __device__ __forceinline__ float2 to_float2(uint32_t w) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+    static __device__ __forceinline__ uint32_t from_float2(float a, float b) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float largest() { return __uint_as_float(0x7f7f0000u); }
+};
+
+// ---- e4m3 codes ------------------------------------------------------------------------------------------
+
+constexpr int kMinScaleExponent = -100;
+
+// Scale of a row whose largest magnitude has the 16-bit pattern `top`: 2^e for the smallest e >= -100 with
+// value <= 448 * 2^e (448 = 1.75 * 2^8), 1 for zero, NaN for an infinity or a NaN.  *inverse is 1 / scale, exact.
+template <bool BF16>
+__device__ __forceinline__ float row_scale(uint32_t top, float* inverse) {
+    if (top >= Half<BF16>::kInf) {
+        *inverse = __uint_as_float(0x7fffffffu);
+        return *inverse;
+    }
+    if (top == 0) {
+        *inverse = 1.f;
+        return 1.f;
+    }
+    const uint32_t bits = __float_as_uint(Half<BF16>::to_float2(top).x);
+    int e = int(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = max(e, kMinScaleExponent);
+    *inverse = __uint_as_float(uint32_t(127 - e) << 23);
+    return __uint_as_float(uint32_t(127 + e) << 23);
+}
+
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+
+__device__ __forceinline__ float2 decode2(uint32_t codes) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+}  // namespace kvmig

@@ -35,6 +35,7 @@
 #include <vector>
 #include <unistd.h>
 
+#include "kvmig_common.h"
 #include "kvmig_kernels.cuh"
 
 namespace kvmig {
@@ -54,14 +55,6 @@ int fail(int code, const char* fmt, ...) {
     g_err = buf;
     return code;
 }
-
-#define CU_TRY(expr)                                                                       \
-    do {                                                                                   \
-        cudaError_t e_ = (expr);                                                           \
-        if (e_ != cudaSuccess)                                                             \
-            return fail(KVMIG_ECUDA, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e_), \
-                        __FILE__, __LINE__);                                               \
-    } while (0)
 
 constexpr int64_t kMagic = 0x4b564d4947303031LL;  // "KVMIG001"
 // handle words
@@ -100,6 +93,7 @@ struct Counters {
     std::atomic<int64_t> migrate_calls{0}, plan_cache_hits{0}, ns_prepare{0}, ns_validate{0}, ns_order{0}, ns_launch{0}, ns_wait{0};
 };
 Counters g_cnt;
+std::atomic<int64_t> g_cache_launches{0}, g_attention_launches{0};
 
 inline int64_t now_ns() {
     return std::chrono::duration_cast<std::chrono::nanoseconds>(std::chrono::steady_clock::now().time_since_epoch()).count();
@@ -242,6 +236,8 @@ int ensure_device(DeviceState** out, int* dev_out) {
     if (dev_out) *dev_out = dev;
     return 0;
 }
+
+void clear_error() { g_err.clear(); }
 
 int check_shape(const kvmig_pool_shape* s, const char* what) {
     if (!s) return fail(KVMIG_EINVAL, "%s: shape is NULL", what);
@@ -1328,6 +1324,8 @@ int64_t kvmig_get_counter(const char* name) {
     if (!std::strcmp(name, "mapped_peers")) return g_cnt.mapped_peers.load();
     if (!std::strcmp(name, "migrate_calls")) return g_cnt.migrate_calls.load();
     if (!std::strcmp(name, "plan_cache_hits")) return g_cnt.plan_cache_hits.load();
+    if (!std::strcmp(name, "cache_launches")) return g_cache_launches.load();
+    if (!std::strcmp(name, "attention_launches")) return g_attention_launches.load();
     if (!std::strcmp(name, "ns_prepare")) return g_cnt.ns_prepare.load();
     if (!std::strcmp(name, "ns_validate")) return g_cnt.ns_validate.load();
     if (!std::strcmp(name, "ns_order")) return g_cnt.ns_order.load();

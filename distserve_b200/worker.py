@@ -78,14 +78,18 @@ class KVWorker:
 
     # --- pools and handles ---------------------------------------------------------------
     def kv_cache_shape(self, num_blocks: int) -> Tuple[int, int, int, int, int]:
+        extra = capi.SCALE_BYTES if self._quantised() else 0      # a quantised row carries its scale in the last dimension
         return (num_blocks, self.model_config.get_num_layers(self.parallel_config),
                 self.model_config.get_num_heads(self.parallel_config), self.cache_config.block_size,
-                self.model_config.get_head_size())
+                self.model_config.get_head_size() + extra)
+
+    def _quantised(self) -> bool:
+        return getattr(self.cache_config, "kv_format", "model") == "e4m3"
 
     def init_kvcache_and_swap(self, num_gpu_blocks: int, num_cpu_blocks: int) -> Tuple[cudaMemoryIpcHandle, cudaMemoryIpcHandle]:
         """Allocate the GPU pools and the pinned host pools, return the K and V
         pool handles (distserve/worker.py:101-134)."""
-        dtype = self.model_config.get_torch_dtype()
+        dtype = torch.uint8 if self._quantised() else self.model_config.get_torch_dtype()
         with torch.cuda.device(self.device):
             self.k_cache = torch.empty(self.kv_cache_shape(num_gpu_blocks), dtype=dtype, device=self.device)
             self.v_cache = torch.empty(self.kv_cache_shape(num_gpu_blocks), dtype=dtype, device=self.device)
@@ -168,6 +172,38 @@ class KVWorker:
 
     def migrate_wait(self, ticket: int) -> None:
         capi.migrate_wait(ticket)
+
+    # --- the cache's contents --------------------------------------------------------------
+    # One layer (counted within this worker) at a time, as a model's forward does.  `starts`, `seq_lens` and
+    # `block_tables` are int32 tensors on this worker's device: sequence i has rows starts[i] .. starts[i + 1] - 1 of
+    # the packed tensors and blocks block_tables[i].  Everything runs on the current stream and nothing is awaited.
+    def write_kv(self, layer: int, k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                 starts: torch.Tensor) -> None:
+        """Put new tokens' K and V, [rows, heads, head_dim], into the pools; `seq_lens` counts them in."""
+        torch.ops.kv_cache_ops.write(k, v, self.k_cache, self.v_cache, layer, block_tables, seq_lens, starts)
+
+    def read_kv(self, layer: int, block_tables: torch.Tensor, starts: torch.Tensor, num_rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The first starts[i + 1] - starts[i] tokens of each sequence, packed, in the model's type; `num_rows` is starts[-1]."""
+        shape = (num_rows, self.k_cache.shape[2], self.model_config.get_head_size())
+        k, v = (torch.empty(shape, dtype=self.model_config.get_torch_dtype(), device=self.device) for _ in range(2))
+        torch.ops.kv_cache_ops.read(self.k_cache, self.v_cache, layer, block_tables, starts, k, v)
+        return k, v
+
+    def attend(self, layer: int, q: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, starts: torch.Tensor,
+               max_rows: int, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of the new tokens' queries, [rows, query heads, head_dim], over the pools (the tokens' own K
+        and V included, see :meth:`write_kv`); no sequence has more than `max_rows` of them."""
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+        torch.ops.kv_attention_ops.paged(q, self.k_cache, self.v_cache, layer, block_tables, seq_lens, starts, max_rows,
+                                         q.shape[-1] ** -0.5 if scale is None else scale, out)
+        return out
+
+    def attend_prompts(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, max_rows: int,
+                       scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of whole packed prompts among themselves, without the pools."""
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+        torch.ops.kv_attention_ops.prompt(q, k, v, starts, max_rows, q.shape[-1] ** -0.5 if scale is None else scale, out)
+        return out
 
     # --- swapping ------------------------------------------------------------------------
     def swap_blocks(self, request_ids: Iterable, source_block_ids: List[int], target_block_ids: List[int],

@@ -257,6 +257,120 @@ KVMIG_API int kvmig_swap(const int64_t* source_block_ids, int64_t num_source,
                void* stream);
 
 /*
+ * ---- The cache's contents: writing, reading, attention ----------------------
+ *
+ * One layer of a K pool and a V pool, the new tokens' rows outside it, and the
+ * attention that reads them.  (The reference keeps these in SwiftTransformer's
+ * model code, which is not part of it.)  All of them enqueue on `stream` and
+ * return without waiting, allocate nothing, and can be captured into a CUDA
+ * graph: every size is a host argument, everything that changes from step to
+ * step (block tables, lengths, row numbers) is read from device memory when the
+ * kernels run.  Pointers belong to the current device.
+ *
+ * A pool holds either the 16-bit type of the rows (shape.elem_size 2), or
+ * quantised values (elem_size 1).  A quantised pool's shape has
+ * head_dim + KVMIG_SCALE_BYTES as its last dimension and the bytes of one
+ * (block, layer, head) are
+ *   block_size rows of head_dim e4m3 codes | block_size scales, 32-bit floats;
+ * value = code * scale.  A scale is the smallest power of two 2^e, e >= -100,
+ * for which no value of the row exceeds 448 * 2^e (1 for a row of zeros), so
+ * the division by it is exact and only the rounding to e4m3 (to nearest, ties
+ * to even) loses anything.  A row that holds an infinity or a NaN has a NaN as its scale
+ * and reads back as NaN.  Migration and swap move such a pool like any other:
+ * the scales travel inside it.
+ *
+ * Conditions that hold for all of them: head_dim as listed at each function;
+ * block_size any positive number, for quantised pools a multiple of 4; strides
+ * in elements and multiples of 8, addresses multiples of 16 bytes; buffers that
+ * are written overlap no other argument.
+ *
+ * Device-side arguments cannot be refused before the launch.  The kernels check
+ * them instead and never access memory outside the arguments:
+ *   - `starts` does not decrease; a sequence whose rows starts[i] .. starts[i+1]
+ *     run backwards or do not lie in [0, num_rows] is skipped;
+ *   - a position whose block id is outside the pool, or that lies beyond
+ *     max_blocks * block_size, is not written by kvmig_cache_write, reads as NaN
+ *     in kvmig_cache_read, and makes every row of kvmig_paged_attention that
+ *     attends to it NaN (other rows of that sequence may become NaN too);
+ *   - the rows of a sequence that has more of them than max_rows become NaN.
+ * Rows that no sequence names are left as they were.
+ */
+enum { KVMIG_F16 = 0, KVMIG_BF16 = 1 };   /* the 16-bit type of rows and of pools with elem_size 2 */
+#define KVMIG_SCALE_BYTES 4               /* bytes per row that a quantised pool's shape carries for the scale */
+
+/* Rows of tokens, [num_rows, num_heads, head_dim], innermost contiguous. */
+typedef struct kvmig_rows {
+    void* data;
+    int64_t num_heads;
+    int64_t row_stride;    /* elements from one token to the next */
+    int64_t head_stride;   /* elements from one head to the next */
+} kvmig_rows;
+
+/* The sequences of a batch.  The arrays are in device memory. */
+typedef struct kvmig_batch {
+    int64_t num_seqs;
+    int64_t num_rows;              /* rows that the row buffers hold */
+    int64_t max_rows;              /* no sequence has more rows than this */
+    const int32_t* starts;         /* [num_seqs + 1]: sequence i has rows starts[i] .. starts[i+1] - 1 */
+    const int32_t* seq_lens;       /* [num_seqs]: its tokens in the cache, those rows included (its last ones) */
+    const int32_t* block_tables;   /* [num_seqs, table_stride]: its blocks, in order */
+    int64_t table_stride;          /* entries from one sequence's table to the next */
+    int64_t max_blocks;            /* entries of a table, at most table_stride */
+} kvmig_batch;
+
+/*
+ * Put new tokens' K and V rows into one layer of the pools: row starts[i] + t
+ * goes to position seq_lens[i] - (starts[i+1] - starts[i]) + t of sequence i;
+ * negative positions are skipped.  head_dim: a multiple of 16, at most 256.  A
+ * slot must not be named twice in one call: which row it then holds is not
+ * defined.  max_rows is not used.
+ */
+KVMIG_API int kvmig_cache_write(const kvmig_rows* k, const kvmig_rows* v, int dtype, void* k_cache, void* v_cache,
+                                const kvmig_pool_shape* shape, int64_t layer, const kvmig_batch* batch, void* stream);
+
+/*
+ * The way back: row starts[i] + t becomes position t of sequence i, for both K
+ * and V, dequantised where the pool is quantised (values beyond the 16-bit
+ * type's largest become that).  head_dim as above.  seq_lens and max_rows are
+ * not used.
+ */
+KVMIG_API int kvmig_cache_read(void* k_cache, void* v_cache, const kvmig_pool_shape* shape, int64_t layer,
+                               const kvmig_batch* batch, const kvmig_rows* k_out, const kvmig_rows* v_out, int dtype,
+                               void* stream);
+
+/*
+ * Causal attention of each sequence's rows over its cache, one layer: row t of
+ * sequence i, at position p = seq_lens[i] - (starts[i+1] - starts[i]) + t, is
+ *   out = sum_j softmax_j(scale * q . k_j) v_j   over the positions j <= p.
+ * The rows' own K and V are in the cache already (kvmig_cache_write).  A row
+ * without a position (p < 0) becomes zeros.  Query head h reads KV head
+ * h / (q heads / KV heads); the KV heads are the pool's.  head_dim: 64 or 128.
+ * scale: finite.  Cached values of the positions that a row's sequence has are
+ * finite; what the pool holds elsewhere does not matter.  Scores, softmax and
+ * sums are in 32 bits; probabilities are rounded to the 16-bit type for the
+ * second product.
+ *
+ * `workspace` is device memory for the partial results of sequences that are
+ * read by several blocks: kvmig_paged_attention_workspace() bytes (0 is a
+ * possible answer; the same arguments give the same number), 16-byte aligned,
+ * contents arbitrary, in use until the call's work on the stream is over.  Two
+ * calls that may run at the same time, two graphs for instance, need two.
+ */
+KVMIG_API int64_t kvmig_paged_attention_workspace(const kvmig_pool_shape* shape, int64_t num_q_heads, const kvmig_batch* batch);
+KVMIG_API int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype, void* k_cache, void* v_cache,
+                                    const kvmig_pool_shape* shape, int64_t layer, const kvmig_batch* batch, double scale,
+                                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention of whole packed prompts, before or without a cache: the rows
+ * of sequence i attend to the rows of sequence i up to their own.  Of `batch`
+ * only num_seqs, num_rows, max_rows and starts are used.  Types, heads,
+ * head_dim, scale and arithmetic as above.
+ */
+KVMIG_API int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig_rows* v, const kvmig_rows* out,
+                                     int dtype, int64_t head_dim, const kvmig_batch* batch, double scale, void* stream);
+
+/*
  * Tuning and introspection (no counterpart in the reference).
  *   options : "kernel" 0 auto | 1 vector loads | 2 bulk-copy pipeline,
  *             "chunk_bytes" size of one work unit = one shared-memory stage
@@ -293,7 +407,8 @@ KVMIG_API int kvmig_swap(const int64_t* source_block_ids, int64_t num_source,
  *   counters: "kernel_launches", "memcpy_calls", "bytes_migrated",
  *             "bytes_swapped", "mapped_peers", "migrate_calls",
  *             "plan_cache_hits" (calls that reused the previous call's
- *             planning), and the host time of the migration entry points by
+ *             planning), "cache_launches" and "attention_launches" (kernels of
+ *             kvmig_cache_* and kvmig_*_attention), and the host time of the migration entry points by
  *             segment, in nanoseconds summed over calls: "ns_prepare"
  *             (arguments to launch descriptors), "ns_validate" (block ids),
  *             "ns_order" (may the launch overlap its predecessors?),
