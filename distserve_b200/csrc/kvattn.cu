@@ -4,26 +4,14 @@
 //
 // in one pass over the keys: when the running maximum grows from m to m', what has been summed so far is multiplied
 // by exp(m - m').
-#include "kvcache_device.cuh"
+#include "kvattn_few.cuh"
 #include "kvmig_common.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace kvmig {
 namespace {
-
-struct AttnRows {
-    char* data;
-    int64_t row_stride, head_stride;   // bytes
-};
-
-struct AttnParams {
-    AttnRows q, out, k, v;             // k, v: whole prompts only
-    CacheView cache;
-    BatchView batch;
-    int32_t heads, group;              // query heads, query heads per KV head
-    float scale_log2;                  // scale * log2(e): exponentials are taken to base 2
-};
 
 constexpr int kWarps = 4;
 
@@ -110,21 +98,77 @@ void launch_simple(const AttnParams& p, bool paged, bool e4m3, unsigned grid, cu
     else attend_simple<HD, BF16, true, true><<<grid, kWarps * 32, 0, stream>>>(p);
 }
 
-int attend(AttnParams& p, bool paged, bool e4m3, int64_t head_dim, int dtype, const kvmig_batch* batch, cudaStream_t stream, const char* what) {
-    p.batch = BatchView{batch->starts, batch->seq_lens, batch->block_tables, batch->table_stride, (int32_t)batch->num_seqs,
-                        (int32_t)batch->num_rows, (int32_t)batch->max_rows, (int32_t)batch->max_blocks};
-    int dev;
-    CU_TRY(cudaGetDevice(&dev));
-    if (batch->num_rows == 0 || batch->num_seqs == 0) return 0;
-    const int64_t grid = (batch->num_rows * p.heads + kWarps - 1) / kWarps;
+// Blocks that the device holds at once when two share an SM (B200: 148 SMs).
+constexpr int64_t kResident = 2 * 148;
+
+// Up to 16 rows of a sequence share a KV head: the kernel for few rows.
+bool few_rows(int64_t max_rows, int64_t group) { return max_rows * group <= kFewRows; }
+
+// Parts that a sequence's keys are cut into: as many as fill the device, but none shorter than 256 keys of what the
+// block tables have room for.
+int64_t splits_for(int64_t tiles, int64_t capacity) {
+    const int64_t fill = kResident / std::max<int64_t>(tiles, 1), longest = std::max<int64_t>(capacity / 256, 1);
+    return std::max<int64_t>(1, std::min(std::min(fill, longest), (int64_t)256));
+}
+
+struct PagedPlan {
+    bool few;
+    int64_t splits, workspace;
+};
+
+PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_batch* b) {
+    PagedPlan plan = {};
+    plan.few = few_rows(b->max_rows, heads / shape->num_heads);
+    plan.splits = plan.few ? splits_for(b->num_seqs * shape->num_heads, std::min<int64_t>(b->max_blocks * shape->block_size, INT32_MAX)) : 1;
+    const int64_t head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
+    if (plan.splits > 1) plan.workspace = b->num_rows * heads * plan.splits * (head_dim * 4 + (int64_t)sizeof(float2));
+    return plan;
+}
+
+BatchView batch_view(const kvmig_batch* batch) {
+    return BatchView{batch->starts, batch->seq_lens, batch->block_tables, batch->table_stride, (int32_t)batch->num_seqs,
+                     (int32_t)batch->num_rows, (int32_t)batch->max_rows, (int32_t)batch->max_blocks};
+}
+
+template <int HD, bool BF16, bool E4M3>
+int launch_few(const AttnParams& p, unsigned grid, cudaStream_t stream) {
+    constexpr int smem = FewShape<HD, E4M3>::kShared;
+    CU_TRY(cudaFuncSetAttribute(attend_few<HD, BF16, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attend_few<HD, BF16, E4M3><<<dim3(grid, p.splits), kFewWarps * 32, smem, stream>>>(p);
+    CU_TRY(cudaGetLastError());
+    g_attention_launches++;
+    if (p.splits > 1) {
+        attend_join<HD, BF16><<<(unsigned)(((int64_t)p.batch.num_rows * p.heads + 3) / 4), 128, 0, stream>>>(p);
+        CU_TRY(cudaGetLastError());
+        g_attention_launches++;
+    }
+    return 0;
+}
+
+template <int HD, bool BF16>
+int launch(const AttnParams& p, bool paged, bool e4m3, bool few, cudaStream_t stream, const char* what) {
+    if (few) {
+        const int64_t grid = (int64_t)p.batch.num_seqs * (p.heads / p.group);
+        if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many sequences for one call", what);
+        return e4m3 ? launch_few<HD, BF16, true>(p, (unsigned)grid, stream) : launch_few<HD, BF16, false>(p, (unsigned)grid, stream);
+    }
+    const int64_t grid = ((int64_t)p.batch.num_rows * p.heads + kWarps - 1) / kWarps;
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
-    if (head_dim == 64 && dtype == KVMIG_F16) launch_simple<64, false>(p, paged, e4m3, (unsigned)grid, stream);
-    else if (head_dim == 64) launch_simple<64, true>(p, paged, e4m3, (unsigned)grid, stream);
-    else if (dtype == KVMIG_F16) launch_simple<128, false>(p, paged, e4m3, (unsigned)grid, stream);
-    else launch_simple<128, true>(p, paged, e4m3, (unsigned)grid, stream);
+    launch_simple<HD, BF16>(p, paged, e4m3, (unsigned)grid, stream);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
     return 0;
+}
+
+int attend(AttnParams& p, bool paged, bool e4m3, bool few, int64_t head_dim, int dtype, const kvmig_batch* batch, cudaStream_t stream,
+           const char* what) {
+    p.batch = batch_view(batch);
+    int dev;
+    CU_TRY(cudaGetDevice(&dev));
+    if (batch->num_rows == 0 || batch->num_seqs == 0) return 0;
+    if (head_dim == 64)
+        return dtype == KVMIG_F16 ? launch<64, false>(p, paged, e4m3, few, stream, what) : launch<64, true>(p, paged, e4m3, few, stream, what);
+    return dtype == KVMIG_F16 ? launch<128, false>(p, paged, e4m3, few, stream, what) : launch<128, true>(p, paged, e4m3, few, stream, what);
 }
 
 AttnRows view(const kvmig_rows* r) { return AttnRows{static_cast<char*>(r->data), r->row_stride * 2, r->head_stride * 2}; }
@@ -155,10 +199,13 @@ int64_t kvmig_paged_attention_workspace(const kvmig_pool_shape* shape, int64_t n
     int rc = check_shape(shape, "paged_attention_workspace");
     if (!rc) rc = check_batch(batch, false, false, "paged_attention_workspace");
     if (rc) return rc;
+    if (batch->max_blocks < 0 || batch->max_blocks > INT32_MAX || shape->block_size > (1 << 16) || shape->num_heads > (1 << 16) ||
+        num_q_heads > (1 << 16))
+        return fail(KVMIG_ELIMIT, "paged_attention_workspace: max_blocks, block_size or heads out of range");
     if (num_q_heads <= 0 || num_q_heads % shape->num_heads)
         return fail(KVMIG_EINVAL, "paged_attention_workspace: %lld query heads do not split over %lld KV heads", (long long)num_q_heads,
                     (long long)shape->num_heads);
-    return 0;
+    return plan_paged(shape, num_q_heads, batch).workspace;
 }
 
 int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype, void* k_cache, void* v_cache,
@@ -187,7 +234,11 @@ int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype,
     p.heads = (int32_t)q->num_heads;
     p.group = (int32_t)(q->num_heads / shape->num_heads);
     p.scale_log2 = (float)(scale * 1.4426950408889634);
-    return attend(p, true, e4m3, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
+    const PagedPlan plan = plan_paged(shape, q->num_heads, batch);
+    p.splits = (int32_t)plan.splits;
+    p.part_out = static_cast<float*>(workspace);
+    p.part_stat = reinterpret_cast<float2*>(p.part_out + batch->num_rows * q->num_heads * plan.splits * head_dim);
+    return attend(p, true, e4m3, plan.few, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
 }
 
 int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig_rows* v, const kvmig_rows* out, int dtype,
@@ -211,7 +262,8 @@ int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig
     p.heads = (int32_t)q->num_heads;
     p.group = (int32_t)(q->num_heads / k->num_heads);
     p.scale_log2 = (float)(scale * 1.4426950408889634);
-    return attend(p, false, false, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
+    p.splits = 1;
+    return attend(p, false, false, false, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
 }
 
 }  // extern "C"

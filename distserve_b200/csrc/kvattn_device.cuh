@@ -1,0 +1,95 @@
+// What the attention kernels share: their parameters, and wrappers of the instructions they use.
+#pragma once
+
+#include "kvcache_device.cuh"
+
+namespace kvmig {
+
+struct AttnRows {
+    char* data;
+    int64_t row_stride, head_stride;   // bytes
+};
+
+struct AttnParams {
+    AttnRows q, out, k, v;             // k, v: whole prompts only
+    CacheView cache;
+    BatchView batch;
+    int32_t heads, group;              // query heads, query heads per KV head
+    float scale_log2;                  // scale * log2(e): exponentials are taken to base 2
+    int32_t splits;                    // parts that a sequence's keys may be cut into, and their partial results:
+    float* part_out;                   // [row][head][split][head_dim], sums before the division
+    float2* part_stat;                 // [row][head][split]: running maximum (base 2) and sum
+};
+
+// Keys of one sequence that split s reads: whole units of kSplitKeys, dealt evenly; later splits may have none.
+constexpr int kSplitKeys = 64;
+struct KeyRange {
+    int begin, end;
+};
+__device__ __forceinline__ KeyRange split_range(int keys, int splits, int s) {
+    const int units = (keys + kSplitKeys - 1) / kSplitKeys, per = (units + splits - 1) / splits;
+    const int64_t begin = (int64_t)s * per * kSplitKeys;
+    KeyRange r;
+    r.begin = (int)min(begin, (int64_t)keys);
+    r.end = (int)min(begin + (int64_t)per * kSplitKeys, (int64_t)keys);
+    return r;
+}
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes (or 4) from global to shared memory without a register in between; zeros where `valid` is false, and then
+// nothing is read.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+    return x;
+}
+// Four 8x8 matrices of 16-bit values, transposed on the way into registers.
+__device__ __forceinline__ uint4 load_matrices_transposed(uint32_t row) {
+    uint4 x;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(row) : "memory");
+    return x;
+}
+
+// d += a b for a 16 x 16 tile a, a 16 x 8 tile b and 32-bit sums.
+template <bool BF16>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two e4m3 codes (the low 16 bits) as two 16-bit values; exact.
+template <bool BF16>
+__device__ __forceinline__ uint32_t widen2(uint32_t codes) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
+    if (!BF16) return w;
+    const float2 f = Half<false>::to_float2(w);
+    return Half<true>::from_float2(f.x, f.y);
+}
+
+__device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fffffffu); }
+
+}  // namespace kvmig

@@ -69,6 +69,12 @@ __host__ __device__ __forceinline__ int block_of(const BatchView& b, const Cache
     return (unsigned)id < (unsigned)c.num_blocks ? id : -1;
 }
 
+// Tokens that a table has room for (kept below 2^31 so that positions rounded up to a tile still fit 32 bits).
+__host__ __device__ __forceinline__ int capacity(const BatchView& b, const CacheView& c) {
+    const int64_t n = (int64_t)b.max_blocks * c.block_size;
+    return n < 0x7fff0000 ? (int)n : 0x7fff0000;
+}
+
 // ---- 16-bit types ----------------------------------------------------------------------------------------
 
 template <bool BF16> struct Half;
