@@ -5,6 +5,7 @@
 // in one pass over the keys: when the running maximum grows from m to m', what has been summed so far is multiplied
 // by exp(m - m').
 #include "kvattn_few.cuh"
+#include "kvattn_tile.cuh"
 #include "kvmig_common.h"
 
 #include <algorithm>
@@ -12,91 +13,6 @@
 
 namespace kvmig {
 namespace {
-
-constexpr int kWarps = 4;
-
-// One warp per row and query head, one key at a time.
-template <int HD, bool BF16, bool PAGED, bool E4M3>
-__global__ void __launch_bounds__(kWarps * 32) attend_simple(const __grid_constant__ AttnParams p) {
-    using H = Half<BF16>;
-    constexpr int N = HD / 64;         // pairs of values that a lane holds
-    const int64_t warp = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, head = (int)(warp % p.heads);
-    const int64_t row64 = warp / p.heads;
-    if (row64 >= p.batch.num_rows) return;
-    const int row = (int)row64, i = find_sequence(p.batch.starts, p.batch.num_seqs, row);
-    const Sequence s = sequence_at(p.batch, i);
-    if (!s.valid || row < s.first || row - s.first >= s.rows) return;
-    const int64_t last = PAGED ? (int64_t)p.batch.seq_lens[i] - s.rows + (row - s.first) : row - s.first;
-    float2 q[N], o[N];
-    const char* qp = p.q.data + row * p.q.row_stride + head * p.q.head_stride;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        q[n] = H::to_float2(reinterpret_cast<const uint32_t*>(qp)[lane * N + n]);
-        o[n] = make_float2(0.f, 0.f);
-    }
-    float m = -INFINITY, l = 0.f;
-    bool bad = s.rows > p.batch.max_rows;
-    const int kv_head = head / p.group;
-    for (int64_t j = 0; j <= last && !bad; ++j) {
-        float2 k[N], v[N];
-        if (PAGED) {
-            const int id = j <= INT32_MAX ? block_of(p.batch, p.cache, i, (int)j) : -1;
-            if (id < 0) { bad = true; break; }
-            const int off = (int)(j % p.cache.block_size);
-            const int64_t tile = id * p.cache.block_stride + (int64_t)kv_head * p.cache.head_stride;
-            if (E4M3) {
-                const int64_t at = tile + off * HD + lane * N * 2, sc = tile + p.cache.block_size * HD + off * 4;
-                const float ks = *reinterpret_cast<const float*>(p.cache.k + sc), vs = *reinterpret_cast<const float*>(p.cache.v + sc);
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    k[n] = decode2(reinterpret_cast<const uint16_t*>(p.cache.k + at)[n]);
-                    v[n] = decode2(reinterpret_cast<const uint16_t*>(p.cache.v + at)[n]);
-                    k[n].x *= ks; k[n].y *= ks; v[n].x *= vs; v[n].y *= vs;
-                }
-            } else {
-                const int64_t at = tile + off * HD * 2 + lane * N * 4;
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    k[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.cache.k + at)[n]);
-                    v[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.cache.v + at)[n]);
-                }
-            }
-        } else {
-            const int64_t r = s.first + j;
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                k[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.k.data + r * p.k.row_stride + kv_head * p.k.head_stride)[lane * N + n]);
-                v[n] = H::to_float2(reinterpret_cast<const uint32_t*>(p.v.data + r * p.v.row_stride + kv_head * p.v.head_stride)[lane * N + n]);
-            }
-        }
-        float dot = 0.f;
-#pragma unroll
-        for (int n = 0; n < N; ++n) dot += q[n].x * k[n].x + q[n].y * k[n].y;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-        dot *= p.scale_log2;
-        const float top = fmaxf(m, dot), keep = exp2f(m - top), e = exp2f(dot - top);
-        m = top;
-        l = l * keep + e;
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            o[n].x = o[n].x * keep + e * v[n].x;
-            o[n].y = o[n].y * keep + e * v[n].y;
-        }
-    }
-    const float inv = bad ? __uint_as_float(0x7fffffffu) : l > 0.f ? 1.f / l : 0.f;
-    uint32_t* op = reinterpret_cast<uint32_t*>(p.out.data + row * p.out.row_stride + head * p.out.head_stride);
-#pragma unroll
-    for (int n = 0; n < N; ++n) op[lane * N + n] = H::from_float2(o[n].x * inv, o[n].y * inv);
-}
-
-template <int HD, bool BF16>
-void launch_simple(const AttnParams& p, bool paged, bool e4m3, unsigned grid, cudaStream_t stream) {
-    if (!paged) attend_simple<HD, BF16, false, false><<<grid, kWarps * 32, 0, stream>>>(p);
-    else if (!e4m3) attend_simple<HD, BF16, true, false><<<grid, kWarps * 32, 0, stream>>>(p);
-    else attend_simple<HD, BF16, true, true><<<grid, kWarps * 32, 0, stream>>>(p);
-}
 
 // Blocks that the device holds at once when two share an SM (B200: 148 SMs).
 constexpr int64_t kResident = 2 * 148;
@@ -119,7 +35,13 @@ struct PagedPlan {
 PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_batch* b) {
     PagedPlan plan = {};
     plan.few = few_rows(b->max_rows, heads / shape->num_heads);
-    plan.splits = plan.few ? splits_for(b->num_seqs * shape->num_heads, std::min<int64_t>(b->max_blocks * shape->block_size, INT32_MAX)) : 1;
+    const int64_t capacity = std::min<int64_t>(b->max_blocks * shape->block_size, INT32_MAX);
+    if (plan.few) {
+        plan.splits = splits_for(b->num_seqs * shape->num_heads, capacity);
+    } else {
+        const int64_t tiles = (b->num_rows * (heads / shape->num_heads) / kBlockRows + b->num_seqs) * shape->num_heads;
+        plan.splits = splits_for(2 * tiles, capacity);        // a block has an SM to itself
+    }
     const int64_t head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
     if (plan.splits > 1) plan.workspace = b->num_rows * heads * plan.splits * (head_dim * 4 + (int64_t)sizeof(float2));
     return plan;
@@ -137,24 +59,38 @@ int launch_few(const AttnParams& p, unsigned grid, cudaStream_t stream) {
     attend_few<HD, BF16, E4M3><<<dim3(grid, p.splits), kFewWarps * 32, smem, stream>>>(p);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
-    if (p.splits > 1) {
-        attend_join<HD, BF16><<<(unsigned)(((int64_t)p.batch.num_rows * p.heads + 3) / 4), 128, 0, stream>>>(p);
-        CU_TRY(cudaGetLastError());
-        g_attention_launches++;
-    }
+    return 0;
+}
+
+template <int HD, bool BF16, bool PAGED, bool E4M3>
+int launch_tiles(const AttnParams& p, cudaStream_t stream, const char* what) {
+    constexpr int smem = TileShape<HD, E4M3>::kShared;
+    const int64_t tiles = ((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group + kBlockRows - 1) / kBlockRows;
+    const int64_t grid = std::max<int64_t>(tiles, 1) * (p.heads / p.group) * p.batch.num_seqs;
+    if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
+    CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attend_tiles<HD, BF16, PAGED, E4M3><<<dim3((unsigned)grid, p.splits), kTileThreads, smem, stream>>>(p);
+    CU_TRY(cudaGetLastError());
+    g_attention_launches++;
     return 0;
 }
 
 template <int HD, bool BF16>
 int launch(const AttnParams& p, bool paged, bool e4m3, bool few, cudaStream_t stream, const char* what) {
+    int rc;
     if (few) {
         const int64_t grid = (int64_t)p.batch.num_seqs * (p.heads / p.group);
         if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many sequences for one call", what);
-        return e4m3 ? launch_few<HD, BF16, true>(p, (unsigned)grid, stream) : launch_few<HD, BF16, false>(p, (unsigned)grid, stream);
+        rc = e4m3 ? launch_few<HD, BF16, true>(p, (unsigned)grid, stream) : launch_few<HD, BF16, false>(p, (unsigned)grid, stream);
+    } else if (!paged) {
+        rc = launch_tiles<HD, BF16, false, false>(p, stream, what);
+    } else {
+        rc = e4m3 ? launch_tiles<HD, BF16, true, true>(p, stream, what) : launch_tiles<HD, BF16, true, false>(p, stream, what);
     }
-    const int64_t grid = ((int64_t)p.batch.num_rows * p.heads + kWarps - 1) / kWarps;
+    if (rc || p.splits == 1) return rc;
+    const int64_t grid = ((int64_t)p.batch.num_rows * p.heads + 3) / 4;
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
-    launch_simple<HD, BF16>(p, paged, e4m3, (unsigned)grid, stream);
+    attend_join<HD, BF16><<<(unsigned)grid, 128, 0, stream>>>(p);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
     return 0;
@@ -188,6 +124,12 @@ int check_attention(const kvmig_rows* q, const kvmig_rows* out, int64_t head_dim
 }
 
 }  // namespace
+
+int64_t attention_timeouts() {
+    unsigned n = 0;
+    return cudaMemcpyFromSymbol(&n, g_attention_timeouts, sizeof n) == cudaSuccess ? (int64_t)n : -1;
+}
+
 }  // namespace kvmig
 
 using namespace kvmig;

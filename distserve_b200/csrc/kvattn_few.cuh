@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) attend_few(const __grid_consta
     const int len = min(tokens, capacity(p.batch, p.cache));
     KeyRange range = split_range(len, p.splits, split);
     const bool whole = split_range(len, p.splits, 0).end == len;               // one split has everything
-    if (whole && split > 0) return;
+    if (split > 0 && (whole || range.begin >= len)) return;
     if (too_many) range.end = range.begin;
 
     // Q: lane (quad, c) has rows quad and quad + 8.  16-bit pools: step t, values 32 (t/2) + 8 c + 4 (t%2) + 0..3;

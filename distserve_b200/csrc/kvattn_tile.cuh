@@ -1,0 +1,462 @@
+// Attention of many rows, over the paged cache or over packed prompts, on the 5th-generation tensor cores.
+//
+// A block takes 256 rows (token x query head of a group) of one sequence and KV head as two tiles of 128, and walks over
+// the keys 128 at a time:
+//   S = Q K^T   128 x 128 x head_dim, both operands in shared memory, sums in tensor memory;
+//   P = 2^(scale S - m), rounded to 16 bits, written back over S's columns;
+//   O += P V    128 x head_dim x 128, P from tensor memory, sums in tensor memory.
+// Each tile has a warpgroup with a thread per row for the softmax, so no value crosses threads.  While one tile's
+// softmax runs the tensor core works on the other's products; one thread issues all of them.  The remaining three warps
+// fill a ring of K and V tiles in shared memory with cp.async, which follows any block size and any strides and
+// leaves keys that are not there as zeros.  Quantised pools pass through a second ring of bytes and are widened
+// to 16 bits by the warps that loaded them.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the last time; until then P may be as large
+// as 256, which costs no precision.  Tensor memory: S0 S1 O0 O1, 128 columns each.
+#pragma once
+
+#include "kvattn_device.cuh"
+#include "tcgen05.cuh"
+
+namespace kvmig {
+
+constexpr int kTileRows = 128, kTileKeys = 128, kBlockRows = 2 * kTileRows;
+constexpr int kSoftmaxThreads = 256, kLoadWarps = 3, kTileThreads = kSoftmaxThreads + kLoadWarps * 32 + 32;
+constexpr float kLazy = 8.f;                 // the maximum may lag behind by this many powers of two
+
+template <int HD, bool E4M3> struct TileShape {
+    static constexpr int kSlot = kTileKeys * HD * 2;                        // a 16-bit tile of K, V or Q
+    static constexpr int kSlots = E4M3 ? 3 : 5;
+    static constexpr int kRawSlot = E4M3 ? kTileKeys * (HD + 4) : 0;        // codes, then scales
+    static constexpr int kRawSlots = E4M3 ? 3 : 0;
+    static constexpr int kBarriers = 2 * kSlots + 1 + 6 + 1;
+    static constexpr int kRing = 2 * kSlot, kRaw = kRing + kSlots * kSlot, kBars = kRaw + kRawSlots * kRawSlot;
+    static constexpr int kShared = kBars + kBarriers * 8 + 32 + 1024;       // and room to align the start to 1024
+};
+
+// 16 e4m3 codes times their row's scale as 16-bit values: exactly what kvmig_cache_read gives.
+template <bool BF16>
+__device__ __forceinline__ void widen16(const uint4& codes, float scale, uint4& lo, uint4& hi) {
+    const uint32_t in[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint32_t out[8];
+    if (!BF16 && scale >= 5.9604644775390625e-08f && scale <= 128.f) {
+        // the scale is a 16-bit value itself and no product leaves the range
+        const __half2 s = __float2half2_rn(scale);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t w = widen2<false>(in[j / 2] >> (j % 2 * 16));
+            const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&w), s);
+            out[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    } else {
+        using H = Half<BF16>;
+        const float top = H::largest();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float2 f = decode2(in[j / 2] >> (j % 2 * 16));
+            f.x *= scale;
+            f.y *= scale;
+            f.x = f.x > top ? top : f.x < -top ? -top : f.x;
+            f.y = f.y > top ? top : f.y < -top ? -top : f.y;
+            out[j] = H::from_float2(f.x, f.y);
+        }
+    }
+    lo = make_uint4(out[0], out[1], out[2], out[3]);
+    hi = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+// Byte offset of 16-byte piece j of row r in a tile: columns of 64 values, 128-byte rows, swizzled.
+__device__ __forceinline__ uint32_t tile_offset(int r, int j) {
+    return (uint32_t)((j >> 3) * (kTileKeys * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4));
+}
+
+__device__ unsigned int g_attention_timeouts;      // blocks that gave up waiting
+
+template <int HD, bool BF16, bool PAGED, bool E4M3>
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_constant__ AttnParams p) {
+    using T = TileShape<HD, E4M3>;
+    using H = Half<BF16>;
+    constexpr int kPieces = HD / 8;                    // 16-byte pieces of a 16-bit row
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + (1024 - (shared_address(smem_raw) & 1023)) % 1024;
+    const uint32_t base = shared_address(smem);
+    const uint32_t bars = base + T::kBars;
+    auto full = [&](int s) { return bars + s * 8; };
+    auto empty = [&](int s) { return bars + (T::kSlots + s) * 8; };
+    const uint32_t q_full = bars + 2 * T::kSlots * 8, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16, drained = pv_done + 16;
+    volatile int* flags = reinterpret_cast<volatile int*>(smem + T::kBars + T::kBarriers * 8);    // failed, bad, tensor memory
+
+    // Which rows and keys.  Later row tiles, which have more keys, come first.
+    const int kv_heads = p.heads / p.group;
+    const int tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
+    const int kv_head = blockIdx.x % kv_heads, seq = blockIdx.x / kv_heads % p.batch.num_seqs;
+    const int tile = tiles - 1 - blockIdx.x / (kv_heads * p.batch.num_seqs), split = blockIdx.y;
+    const Sequence s = sequence_at(p.batch, seq);
+    const int64_t total = (int64_t)s.rows * p.group, row0 = (int64_t)tile * kBlockRows;
+    if (row0 >= total) return;
+    if (s.rows > p.batch.max_rows) {                   // more rows than the grid has tiles for
+        if (tile == 0 && split == 0)
+            for (int64_t x = threadIdx.x; x < total * (HD / 8); x += kTileThreads) {
+                const int64_t r = x / (HD / 8);
+                *reinterpret_cast<uint4*>(p.out.data + (s.first + r / p.group) * p.out.row_stride +
+                                          (kv_head * p.group + r % p.group) * p.out.head_stride + x % (HD / 8) * 16) =
+                    make_uint4(H::kNan2, H::kNan2, H::kNan2, H::kNan2);
+            }
+        return;
+    }
+    const int tokens = PAGED ? max(p.batch.seq_lens[seq], 0) : s.rows, first_pos = tokens - s.rows;
+    const int len = PAGED ? min(tokens, capacity(p.batch, p.cache)) : tokens;
+    const KeyRange range = split_range(len, p.splits, split);
+    const bool whole = split_range(len, p.splits, 0).end == len;
+    if (split > 0 && (whole || range.begin >= len)) return;
+    int n[2];                                          // key tiles of each row tile
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int64_t end = min(row0 + (t + 1) * kTileRows, total);
+        const int keys = end <= row0 + t * kTileRows ? 0 : (int)min((int64_t)range.end, first_pos + (end - 1) / p.group + 1) - range.begin;
+        n[t] = keys > 0 ? (keys + kTileKeys - 1) / kTileKeys : 0;
+    }
+    const int steps = max(n[0], n[1]);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < T::kSlots; ++i) {
+            barrier_init(full(i), kLoadWarps);
+            barrier_init(empty(i), 1);
+        }
+        barrier_init(q_full, kLoadWarps);
+        barrier_init(drained, 1);
+        for (int t = 0; t < 2; ++t) {
+            barrier_init(s_full + t * 8, 1);
+            barrier_init(p_full + t * 8, 4);
+            barrier_init(pv_done + t * 8, 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_shared();
+        flags[0] = 0;
+        flags[1] = tokens > len;                       // the table is too short for the sequence
+    }
+    if (warp == kTileThreads / 32 - 1) tmem_alloc(shared_address(const_cast<int*>(flags + 2)), 512);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = flags[2];
+    // A whole warp waits, and goes on or gives up together.
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(bar, parity, flags)) != 0; };
+    // The sign of the scale is taken by the products and a scale of zero by Q, so that the maximum of the scores is theirs too.
+    const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+
+    if (warp < kSoftmaxThreads / 32) {
+        // ---- softmax: a thread per row -------------------------------------------------------------------
+        const int t = warp >> 2;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;             // this warp's 32 rows of tensor memory
+        const uint32_t s_at = tmem + t * kTileKeys + lanes, o_at = tmem + 2 * kTileKeys + t * 128 + lanes;
+        const int64_t row = row0 + threadIdx.x;
+        const bool there = row < total;
+        const int64_t token = there ? row / p.group : 0;
+        const int last = there ? (int)min(first_pos + token, (int64_t)range.end - 1) : -1;      // last key that the row sees
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int i = 0; i < n[t]; ++i) {
+            if (!(ok = warp_wait(s_full + t * 8, i & 1))) break;
+            tmem_fence_after();
+            const int seen = last - (range.begin + i * kTileKeys);      // columns up to this one count
+            const bool masked = __any_sync(0xffffffffu, seen < kTileKeys - 1);
+            uint32_t b[64];
+            float top = -INFINITY;
+            {
+                uint32_t a[64];
+                tmem_load(a, s_at);
+                if (masked)
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) a[j] = j <= seen ? a[j] : 0xff800000u;
+                float top2 = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 64; j += 2) {
+                    top = fmaxf(top, __uint_as_float(a[j]));
+                    top2 = fmaxf(top2, __uint_as_float(a[j + 1]));
+                }
+                tmem_load(b, s_at + 64);
+                if (masked)
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) b[j] = j + 64 <= seen ? b[j] : 0xff800000u;
+#pragma unroll
+                for (int j = 0; j < 64; j += 2) {
+                    top = fmaxf(top, __uint_as_float(b[j]));
+                    top2 = fmaxf(top2, __uint_as_float(b[j + 1]));
+                }
+                top = fmaxf(top, top2) * scale;
+            }
+            if (i == 0) {
+                m = top;
+            } else {
+                const bool grown = top > m + kLazy;
+                if (__any_sync(0xffffffffu, grown)) {
+                    if (!(ok = warp_wait(pv_done + t * 8, (i - 1) & 1))) break;
+                    tmem_fence_after();
+                    const float keep = grown ? exp2_fast(m - top) : 1.f;
+                    if (grown) m = top;
+                    l *= keep;
+#pragma unroll
+                    for (int j = 0; j < HD; j += 32) {
+                        uint32_t o[32];
+                        tmem_load(o, o_at + j);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tmem_store(o_at + j, o);
+                    }
+                }
+            }
+            const float shift = m == -INFINITY ? 0.f : -m;
+            float sum[4] = {};
+            // Probabilities go where the second half of the scores was: columns 64 .. 127 of S, two to a column.
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) {
+                const float x = exp2_fast(fmaf(__uint_as_float(b[j]), scale, shift));
+                const float y = exp2_fast(fmaf(__uint_as_float(b[j + 1]), scale, shift));
+                sum[j % 4] += x;
+                sum[j % 4 + 1] += y;
+                w[j / 2] = H::from_float2(x, y);
+            }
+            tmem_store(s_at + 96, w);
+            tmem_load(b, s_at);
+            if (masked)
+#pragma unroll
+                for (int j = 0; j < 64; ++j) b[j] = j <= seen ? b[j] : 0xff800000u;
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) {
+                const float x = exp2_fast(fmaf(__uint_as_float(b[j]), scale, shift));
+                const float y = exp2_fast(fmaf(__uint_as_float(b[j + 1]), scale, shift));
+                sum[j % 4] += x;
+                sum[j % 4 + 1] += y;
+                w[j / 2] = H::from_float2(x, y);
+            }
+            tmem_store(s_at + 64, w);
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_wait_store();
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(p_full + t * 8);
+        }
+        __syncwarp();
+        asm volatile("bar.sync 1, 352;" ::: "memory");                  // the loading warps have said what they found
+        if (ok && n[t] > 0) ok = warp_wait(pv_done + t * 8, (n[t] - 1) & 1);
+        tmem_fence_after();
+        if (!ok || flags[0] || flags[1]) l = not_a_number();
+        const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
+        const int64_t out_row = s.first + token, head = kv_head * p.group + (there ? row % p.group : 0);
+        const int64_t part = (out_row * p.heads + head) * p.splits + split;
+        char* to = p.out.data + out_row * p.out.row_stride + head * p.out.head_stride;
+        if (there && !whole) p.part_stat[part] = make_float2(m, l);
+#pragma unroll
+        for (int j = 0; j < HD; j += 32) {
+            uint32_t o[32];
+            __syncwarp();
+            if (n[t] > 0) {
+                tmem_load(o, o_at + j);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0;
+            }
+            if (!there) continue;
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) h[x] = H::from_float2(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv);
+                    *reinterpret_cast<uint4*>(to + (j + e) * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<uint4*>(p.part_out + part * HD + j + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+        }
+        tmem_fence_before();
+    } else if (warp < kSoftmaxThreads / 32 + kLoadWarps) {
+        // ---- loading -------------------------------------------------------------------------------------
+        const int w = warp - kSoftmaxThreads / 32;
+        constexpr int kRowsAtOnce = 32 / kPieces;                       // rows that a warp copies with one instruction
+        for (int g = w; g < kBlockRows / kRowsAtOnce; g += kLoadWarps) {
+            const int r = g * kRowsAtOnce + lane / kPieces, j = lane % kPieces;
+            const int64_t row = row0 + r;
+            const bool there = row < total && p.scale_log2 != 0.f;
+            const char* from = p.q.data;
+            if (there) from += (s.first + row / p.group) * p.q.row_stride + (kv_head * p.group + row % p.group) * p.q.head_stride + j * 16;
+            copy16(base + (r / kTileRows) * T::kSlot + tile_offset(r % kTileRows, j), from, there);
+        }
+        copy_commit();
+        const int count = 2 * steps;                                    // K and V tiles in turn
+        bool bad = false;
+        // Byte offset of four keys of the tile, r = lane + 32 x; -1 if there is no such key.
+        int64_t at_k[4], at_v[4];
+        auto look_up = [&](int i) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int key = range.begin + i * kTileKeys + lane + 32 * x;
+                at_k[x] = at_v[x] = -1;
+                if (key >= range.end) continue;
+                if (PAGED) {
+                    const int id = block_of(p.batch, p.cache, seq, key);
+                    if (id < 0) bad = true;
+                    else
+                        at_k[x] = at_v[x] = id * p.cache.block_stride + (int64_t)kv_head * p.cache.head_stride +
+                                            (E4M3 ? (int64_t)(key % p.cache.block_size) << 40 : (int64_t)(key % p.cache.block_size) * HD * 2);
+                } else {
+                    at_k[x] = (int64_t)(s.first + key) * p.k.row_stride + kv_head * p.k.head_stride;
+                    at_v[x] = (int64_t)(s.first + key) * p.v.row_stride + kv_head * p.v.head_stride;
+                }
+            }
+        };
+        const char* k_data = PAGED ? p.cache.k : p.k.data;
+        const char* v_data = PAGED ? p.cache.v : p.v.data;
+        constexpr int kLag = 2;                                         // tiles in flight behind the newest
+        bool ok = true;
+        if (!E4M3) {
+            for (int c = 0; c < count + kLag; ++c) {
+                if (c < count) {
+                    const int slot = c % T::kSlots;
+                    if (c % 2 == 0) look_up(c / 2);
+                    if (c >= T::kSlots && !(ok = warp_wait(empty(slot), (c / T::kSlots - 1) & 1))) break;
+                    const uint32_t to = base + T::kRing + slot * T::kSlot;
+                    const char* data = c % 2 ? v_data : k_data;
+                    for (int g = w; g < kTileKeys / kRowsAtOnce; g += kLoadWarps) {
+                        const int r = g * kRowsAtOnce + lane / kPieces, j = lane % kPieces;
+                        const int64_t mine = g * kRowsAtOnce < 32 ? (c % 2 ? at_v[0] : at_k[0]) : g * kRowsAtOnce < 64 ? (c % 2 ? at_v[1] : at_k[1])
+                                             : g * kRowsAtOnce < 96 ? (c % 2 ? at_v[2] : at_k[2]) : (c % 2 ? at_v[3] : at_k[3]);
+                        const int64_t at = __shfl_sync(0xffffffffu, mine, r & 31);
+                        copy16(to + tile_offset(r, j), data + (at >= 0 ? at + j * 16 : 0), at >= 0);
+                    }
+                }
+                copy_commit();
+                if (c >= kLag) {
+                    copy_wait<kLag>();
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (c == kLag) barrier_arrive(q_full);
+                        barrier_arrive(full((c - kLag) % T::kSlots));
+                    }
+                }
+            }
+        } else {
+            constexpr int kRowPieces = HD / 16, kRawRows = 32 / kRowPieces;
+            auto fetch = [&](int c) {                                   // codes and scales of tile c into the ring of bytes
+                if (c < count) {
+                    if (c % 2 == 0) look_up(c / 2);
+                    const uint32_t to = base + T::kRaw + c % T::kRawSlots * T::kRawSlot;
+                    const char* data = c % 2 ? v_data : k_data;
+                    for (int g = w; g < kTileKeys / kRawRows; g += kLoadWarps) {
+                        const int r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
+                        const int64_t mine = g * kRawRows < 32 ? at_k[0] : g * kRawRows < 64 ? at_k[1] : g * kRawRows < 96 ? at_k[2] : at_k[3];
+                        const int64_t packed = __shfl_sync(0xffffffffu, mine, r & 31);
+                        const int64_t tile_at = packed & 0xffffffffffll;
+                        const int offset = (int)(packed >> 40);
+                        const bool there = packed >= 0;
+                        copy16(to + r * HD + j * 16, data + (there ? tile_at + offset * HD + j * 16 : 0), there);
+                        if (j == 0) copy4(to + kTileKeys * HD + r * 4, data + (there ? tile_at + (int64_t)p.cache.block_size * HD + offset * 4 : 0), there);
+                    }
+                }
+                copy_commit();
+            };
+            fetch(0);
+            fetch(1);
+            for (int c = 0; c < count; ++c) {
+                fetch(c + 2);
+                copy_wait<2>();
+                __syncwarp();
+                const int slot = c % T::kSlots;
+                if (c >= T::kSlots && !(ok = warp_wait(empty(slot), (c / T::kSlots - 1) & 1))) break;
+                const unsigned char* raw = smem + T::kRaw + c % T::kRawSlots * T::kRawSlot;
+                unsigned char* to = smem + T::kRing + slot * T::kSlot;
+                for (int g = w; g < kTileKeys / kRawRows; g += kLoadWarps) {
+                    const int r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
+                    uint4 lo, hi;
+                    widen16<BF16>(*reinterpret_cast<const uint4*>(raw + r * HD + j * 16), *reinterpret_cast<const float*>(raw + kTileKeys * HD + r * 4), lo, hi);
+                    const int first = j >= kRowPieces / 2;              // half of the lanes store their second piece first: other banks
+                    *reinterpret_cast<uint4*>(to + tile_offset(r, 2 * j + first)) = first ? hi : lo;
+                    *reinterpret_cast<uint4*>(to + tile_offset(r, 2 * j + 1 - first)) = first ? lo : hi;
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    if (c == 0) barrier_arrive(q_full);                 // Q's copies are older than the first tile's
+                    barrier_arrive(full(slot));
+                }
+            }
+        }
+        copy_wait<0>();
+        if (bad) flags[1] = 1;
+        __threadfence_block();
+        __syncwarp();
+        asm volatile("bar.arrive 1, 352;" ::: "memory");
+    } else {
+        // ---- products: one thread issues them all ---------------------------------------------------------
+        if (lane == 0 && steps > 0) {
+            const uint32_t s_kind = product_kind(BF16, kTileRows, kTileKeys, false, false) | (p.scale_log2 < 0.f ? 1u << 13 : 0u);
+            constexpr uint32_t o_kind = product_kind(BF16, kTileRows, HD, true, false);
+            bool ok = barrier_wait(q_full, 0, flags);
+            auto scores = [&](int t, int slot) {
+                const uint32_t k_at = base + T::kRing + slot * T::kSlot, q_at = base + t * T::kSlot;
+#pragma unroll
+                for (int x = 0; x < HD / 16; ++x) {
+                    const uint32_t step = (x / 4) * (kTileKeys * 128) + (x % 4) * 32;
+                    mma_shared(tmem + t * kTileKeys, operand(q_at + step, 16, 1024), operand(k_at + step, 16, 1024), s_kind, x > 0);
+                }
+                mma_commit(s_full + t * 8);
+            };
+            if (ok) ok = barrier_wait(full(0), 0, flags);
+            if (ok) {
+                tmem_fence_after();
+                for (int t = 0; t < 2; ++t)
+                    if (n[t] > 0) scores(t, 0);
+                mma_commit(empty(0));
+            }
+            for (int i = 0; i < steps && ok; ++i) {
+                const int v = 2 * i + 1, k = 2 * i + 2, v_slot = v % T::kSlots, k_slot = k % T::kSlots;
+                ok = barrier_wait(full(v_slot), (v / T::kSlots) & 1, flags);
+                bool k_ready = false;
+                for (int t = 0; t < 2 && ok; ++t) {
+                    if (i >= n[t]) continue;
+                    if (!(ok = barrier_wait(p_full + t * 8, i & 1, flags))) break;
+                    tmem_fence_after();
+                    const uint32_t v_at = base + T::kRing + v_slot * T::kSlot;
+#pragma unroll
+                    for (int x = 0; x < kTileKeys / 16; ++x)
+                        mma_tmem(tmem + 2 * kTileKeys + t * 128, tmem + t * kTileKeys + 64 + x * 8, operand(v_at + x * 2048, kTileKeys * 128, 1024),
+                                 o_kind, i > 0 || x > 0);
+                    mma_commit(pv_done + t * 8);
+                    if (i + 1 < n[t]) {
+                        if (!k_ready) {
+                            if (!(ok = barrier_wait(full(k_slot), (k / T::kSlots) & 1, flags))) break;
+                            tmem_fence_after();
+                            k_ready = true;
+                        }
+                        scores(t, k_slot);
+                    }
+                }
+                if (ok) {
+                    mma_commit(empty(v_slot));
+                    if (k_ready) mma_commit(empty(k_slot));
+                }
+            }
+            if (!ok) {
+                // products still in flight read shared memory and write tensor memory: give them their chance to end
+                atomicAdd(&g_attention_timeouts, 1u);
+                mma_commit(drained);
+                int quiet = 0;
+                barrier_wait(drained, 0, &quiet);
+            }
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    if (warp == kTileThreads / 32 - 1) {
+        tmem_fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+}  // namespace kvmig

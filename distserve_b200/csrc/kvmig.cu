@@ -1326,6 +1326,7 @@ int64_t kvmig_get_counter(const char* name) {
     if (!std::strcmp(name, "plan_cache_hits")) return g_cnt.plan_cache_hits.load();
     if (!std::strcmp(name, "cache_launches")) return g_cache_launches.load();
     if (!std::strcmp(name, "attention_launches")) return g_attention_launches.load();
+    if (!std::strcmp(name, "attention_timeouts")) return attention_timeouts();
     if (!std::strcmp(name, "ns_prepare")) return g_cnt.ns_prepare.load();
     if (!std::strcmp(name, "ns_validate")) return g_cnt.ns_validate.load();
     if (!std::strcmp(name, "ns_order")) return g_cnt.ns_order.load();

@@ -16,6 +16,9 @@ int fail(int code, const char* fmt, ...);
 void clear_error();
 int check_shape(const kvmig_pool_shape* s, const char* what);
 
+// Blocks of the attention kernels on the current device that gave up waiting (their rows are NaN); waits for the device.
+int64_t attention_timeouts();
+
 extern std::atomic<int64_t> g_cache_launches, g_attention_launches;
 
 #define CU_TRY(expr)                                                                       \

@@ -408,7 +408,10 @@ KVMIG_API int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, c
  *             "bytes_swapped", "mapped_peers", "migrate_calls",
  *             "plan_cache_hits" (calls that reused the previous call's
  *             planning), "cache_launches" and "attention_launches" (kernels of
- *             kvmig_cache_* and kvmig_*_attention), and the host time of the migration entry points by
+ *             kvmig_cache_* and kvmig_*_attention), "attention_timeouts"
+ *             (blocks of the attention kernels on the current device whose
+ *             bounded waits ran out, their rows then being NaN; reading it
+ *             waits for the device), and the host time of the migration entry points by
  *             segment, in nanoseconds summed over calls: "ns_prepare"
  *             (arguments to launch descriptors), "ns_validate" (block ids),
  *             "ns_order" (may the launch overlap its predecessors?),
