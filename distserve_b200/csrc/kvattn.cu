@@ -62,14 +62,72 @@ int launch_few(const AttnParams& p, unsigned grid, cudaStream_t stream) {
     return 0;
 }
 
+// The driver's call that makes a map for the copy engine; the library links only the runtime.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled f = [] {
+        void* at = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &at, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            at = nullptr;
+        return reinterpret_cast<EncodeTiled>(at);
+    }();
+    return f;
+}
+
+// Rows of 16-bit values in boxes of 64 values by `box` rows, 128-byte swizzle.  dims: values, [heads,] rows.
+bool encode_map(CUtensorMap* map, const void* data, int rank, const cuuint64_t* dims, const cuuint64_t* strides, int box, bool bf16) {
+    const cuuint32_t boxes[3] = {64, rank == 3 ? 1u : (cuuint32_t)box, (cuuint32_t)box}, steps[3] = {1, 1, 1};
+    return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(data), dims,
+                          strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Maps for this call, or p.box = 0 where the copy engine cannot follow the layout: blocks must tile 128 keys in
+// pieces of whole 1024-byte swizzle groups (8 rows).
+void make_maps(AttnParams& p, AttnMaps& maps, bool paged, bool e4m3, int64_t head_dim, bool bf16) {
+    p.box = 0;
+    if (!paged) {
+        if (!encode_tiled()) return;
+        const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)(p.heads / p.group), (cuuint64_t)p.batch.num_rows};
+        auto strides = [&](const AttnRows& r, cuuint64_t (&s)[2]) {       // the stride of a dimension of one says nothing
+            s[0] = dims[1] > 1 ? r.head_stride : head_dim * 2;
+            s[1] = dims[2] > 1 ? r.row_stride : head_dim * 2;
+        };
+        cuuint64_t ks[2], vs[2];
+        strides(p.k, ks);
+        strides(p.v, vs);
+        if (encode_map(&maps.k, p.k.data, 3, dims, ks, kTileKeys, bf16) && encode_map(&maps.v, p.v.data, 3, dims, vs, kTileKeys, bf16)) p.box = kTileKeys;
+        return;
+    }
+    const int bs = p.cache.block_size;
+    const int box = bs >= kTileKeys ? (bs % kTileKeys == 0 ? kTileKeys : 0) : (bs % 8 == 0 && kTileKeys % bs == 0 ? bs : 0);
+    if (!box || e4m3) {
+        p.box = box;
+        return;
+    }
+    const int kv_heads = p.heads / p.group;
+    const int64_t rows = (int64_t)p.cache.num_blocks * p.layers * kv_heads * bs;
+    if (!encode_tiled() || rows > INT32_MAX) return;
+    const int64_t back = (int64_t)p.layer * kv_heads * p.cache.head_stride;          // from this layer to the pool's start
+    const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)head_dim * 2};
+    if (encode_map(&maps.k, p.cache.k - back, 2, dims, strides, box, bf16) && encode_map(&maps.v, p.cache.v - back, 2, dims, strides, box, bf16)) p.box = box;
+}
+
 template <int HD, bool BF16, bool PAGED, bool E4M3>
-int launch_tiles(const AttnParams& p, cudaStream_t stream, const char* what) {
+int launch_tiles(const AttnParams& params, cudaStream_t stream, const char* what) {
+    AttnParams p = params;
+    AttnMaps maps = {};
+    make_maps(p, maps, PAGED, E4M3, HD, BF16);
     constexpr int smem = TileShape<HD, E4M3>::kShared;
     const int64_t tiles = ((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group + kBlockRows - 1) / kBlockRows;
     const int64_t grid = std::max<int64_t>(tiles, 1) * (p.heads / p.group) * p.batch.num_seqs;
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attend_tiles<HD, BF16, PAGED, E4M3><<<dim3((unsigned)grid, p.splits), kTileThreads, smem, stream>>>(p);
+    attend_tiles<HD, BF16, PAGED, E4M3><<<dim3((unsigned)grid, p.splits), kTileThreads, smem, stream>>>(p, maps);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
     return 0;
@@ -173,6 +231,8 @@ int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype,
     p.cache = CacheView{static_cast<char*>(k_cache) + at_layer, static_cast<char*>(v_cache) + at_layer,
                         shape->num_layers * shape->num_heads * tile, (int32_t)tile, (int32_t)shape->num_blocks,
                         (int32_t)shape->block_size};
+    p.layers = (int32_t)shape->num_layers;
+    p.layer = (int32_t)layer;
     p.heads = (int32_t)q->num_heads;
     p.group = (int32_t)(q->num_heads / shape->num_heads);
     p.scale_log2 = (float)(scale * 1.4426950408889634);

@@ -1,6 +1,8 @@
 // What the attention kernels share: their parameters, and wrappers of the instructions they use.
 #pragma once
 
+#include <cuda.h>
+
 #include "kvcache_device.cuh"
 
 namespace kvmig {
@@ -19,10 +21,17 @@ struct AttnParams {
     int32_t splits;                    // parts that a sequence's keys may be cut into, and their partial results:
     float* part_out;                   // [row][head][split][head_dim], sums before the division
     float2* part_stat;                 // [row][head][split]: running maximum (base 2) and sum
+    int32_t box;                       // keys that the copy engine moves at once; 0: it cannot follow this layout
+    int32_t layers, layer;
+};
+
+// Maps of K and V for the copy engine: rows of head_dim values, copied in boxes of 64 values by up to 128 rows.
+struct AttnMaps {
+    CUtensorMap k, v;
 };
 
 // Keys of one sequence that split s reads: whole units of kSplitKeys, dealt evenly; later splits may have none.
-constexpr int kSplitKeys = 64;
+constexpr int kSplitKeys = 128;
 struct KeyRange {
     int begin, end;
 };

@@ -7,9 +7,10 @@
 //   O += P V    128 x head_dim x 128, P from tensor memory, sums in tensor memory.
 // Each tile has a warpgroup with a thread per row for the softmax, so no value crosses threads.  While one tile's
 // softmax runs the tensor core works on the other's products; one thread issues all of them.  The remaining three warps
-// fill a ring of K and V tiles in shared memory with cp.async, which follows any block size and any strides and
-// leaves keys that are not there as zeros.  Quantised pools pass through a second ring of bytes and are widened
-// to 16 bits by the warps that loaded them.
+// fill a ring of K and V tiles in shared memory: whole tiles through the copy engine, a box per block and 64 values, and
+// what it cannot follow (a sequence's last keys, whose neighbours in the block must become zeros; block sizes that
+// do not tile 128 keys) with cp.async.  Quantised pools pass through a second ring of bytes and are widened to 16 bits
+// by those warps.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time; until then P may be as large
 // as 256, which costs no precision.  Tensor memory: S0 S1 O0 O1, 128 columns each.
@@ -29,7 +30,7 @@ template <int HD, bool E4M3> struct TileShape {
     static constexpr int kSlots = E4M3 ? 3 : 5;
     static constexpr int kRawSlot = E4M3 ? kTileKeys * (HD + 4) : 0;        // codes, then scales
     static constexpr int kRawSlots = E4M3 ? 3 : 0;
-    static constexpr int kBarriers = 2 * kSlots + 1 + 6 + 1;
+    static constexpr int kBarriers = 2 * kSlots + 1 + 6 + 1 + 2 * kRawSlots;
     static constexpr int kRing = 2 * kSlot, kRaw = kRing + kSlots * kSlot, kBars = kRaw + kRawSlots * kRawSlot;
     static constexpr int kShared = kBars + kBarriers * 8 + 32 + 1024;       // and room to align the start to 1024
 };
@@ -73,7 +74,7 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int j) {
 __device__ unsigned int g_attention_timeouts;      // blocks that gave up waiting
 
 template <int HD, bool BF16, bool PAGED, bool E4M3>
-__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_constant__ AttnParams p, const __grid_constant__ AttnMaps maps) {
     using T = TileShape<HD, E4M3>;
     using H = Half<BF16>;
     constexpr int kPieces = HD / 8;                    // 16-byte pieces of a 16-bit row
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
     const uint32_t bars = base + T::kBars;
     auto full = [&](int s) { return bars + s * 8; };
     auto empty = [&](int s) { return bars + (T::kSlots + s) * 8; };
-    const uint32_t q_full = bars + 2 * T::kSlots * 8, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16, drained = pv_done + 16;
+    const uint32_t q_full = bars + 2 * T::kSlots * 8, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16, drained = pv_done + 16, raw_full = drained + 8, raw_empty = raw_full + T::kRawSlots * 8;
     volatile int* flags = reinterpret_cast<volatile int*>(smem + T::kBars + T::kBarriers * 8);    // failed, bad, tensor memory
 
     // Which rows and keys.  Later row tiles, which have more keys, come first.
@@ -126,6 +127,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
         }
         barrier_init(q_full, kLoadWarps);
         barrier_init(drained, 1);
+        for (int i = 0; i < T::kRawSlots; ++i) {
+            barrier_init(raw_full + i * 8, 1);
+            barrier_init(raw_empty + i * 8, kLoadWarps);
+        }
         for (int t = 0; t < 2; ++t) {
             barrier_init(s_full + t * 8, 1);
             barrier_init(p_full + t * 8, 4);
@@ -289,8 +294,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
         }
         copy_commit();
         const int count = 2 * steps;                                    // K and V tiles in turn
-        bool bad = false;
-        // Byte offset of four keys of the tile, r = lane + 32 x; -1 if there is no such key.
+        bool bad = false, ok = true;
+        // Whole tiles go through the copy engine where it can follow the layout; the last one of a sequence, whose
+        // missing keys have to be zeros, and other layouts are copied 16 bytes at a time.
+        auto by_engine = [&](int c) { return p.box > 0 && range.begin + (c / 2 + 1) * kTileKeys <= range.end; };
+        const int boxes = p.box > 0 ? kTileKeys / p.box : 1;
+        // Byte offsets of four keys of a tile, r = lane + 32 x; -1 if there is no such key.
         int64_t at_k[4], at_v[4];
         auto look_up = [&](int i) {
 #pragma unroll
@@ -310,24 +319,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                 }
             }
         };
+        auto of_row = [&](int r, bool is_v) {
+            const int64_t mine = r < 32 ? (is_v ? at_v[0] : at_k[0]) : r < 64 ? (is_v ? at_v[1] : at_k[1]) : r < 96 ? (is_v ? at_v[2] : at_k[2]) : (is_v ? at_v[3] : at_k[3]);
+            return mine;
+        };
         const char* k_data = PAGED ? p.cache.k : p.k.data;
         const char* v_data = PAGED ? p.cache.v : p.v.data;
         constexpr int kLag = 2;                                         // tiles in flight behind the newest
-        bool ok = true;
         if (!E4M3) {
             for (int c = 0; c < count + kLag; ++c) {
                 if (c < count) {
                     const int slot = c % T::kSlots;
-                    if (c % 2 == 0) look_up(c / 2);
-                    if (c >= T::kSlots && !(ok = warp_wait(empty(slot), (c / T::kSlots - 1) & 1))) break;
                     const uint32_t to = base + T::kRing + slot * T::kSlot;
-                    const char* data = c % 2 ? v_data : k_data;
-                    for (int g = w; g < kTileKeys / kRowsAtOnce; g += kLoadWarps) {
-                        const int r = g * kRowsAtOnce + lane / kPieces, j = lane % kPieces;
-                        const int64_t mine = g * kRowsAtOnce < 32 ? (c % 2 ? at_v[0] : at_k[0]) : g * kRowsAtOnce < 64 ? (c % 2 ? at_v[1] : at_k[1])
-                                             : g * kRowsAtOnce < 96 ? (c % 2 ? at_v[2] : at_k[2]) : (c % 2 ? at_v[3] : at_k[3]);
-                        const int64_t at = __shfl_sync(0xffffffffu, mine, r & 31);
-                        copy16(to + tile_offset(r, j), data + (at >= 0 ? at + j * 16 : 0), at >= 0);
+                    if (c >= T::kSlots && !(ok = warp_wait(empty(slot), (c / T::kSlots - 1) & 1))) break;
+                    if (by_engine(c)) {
+                        const void* map = c % 2 ? &maps.v : &maps.k;
+                        const int key = range.begin + c / 2 * kTileKeys;
+                        if (w > 0) {
+                            if (lane == 0) barrier_arrive(full(slot));
+                        } else if (!PAGED) {
+                            if (lane == 0) {
+                                barrier_expect(full(slot), T::kSlot);
+                                for (int h = 0; h < HD / 64; ++h) box_copy(to + h * kTileKeys * 128, map, h * 64, kv_head, s.first + key, full(slot));
+                            }
+                        } else {
+                            const int b = lane / (HD / 64), h = lane % (HD / 64), first = key + b * p.box;
+                            int id = -1;
+                            if (b < boxes) id = block_of(p.batch, p.cache, seq, first);
+                            const bool there = b < boxes && id >= 0;
+                            bad |= b < boxes && id < 0;
+                            const int copies = __popc(__ballot_sync(0xffffffffu, there));
+                            if (lane == 0) barrier_expect(full(slot), copies * p.box * 128);
+                            __syncwarp();
+                            if (there)
+                                box_copy(to + h * kTileKeys * 128 + b * p.box * 128, map, h * 64,
+                                         ((id * p.layers + p.layer) * kv_heads + kv_head) * p.cache.block_size + first % p.cache.block_size, full(slot));
+                        }
+                    } else {
+                        look_up(c / 2);
+                        const char* data = c % 2 ? v_data : k_data;
+                        for (int g = w; g < kTileKeys / kRowsAtOnce; g += kLoadWarps) {
+                            const int r = g * kRowsAtOnce + lane / kPieces, j = lane % kPieces;
+                            const int64_t at = __shfl_sync(0xffffffffu, of_row(g * kRowsAtOnce, c % 2), r & 31);
+                            copy16(to + tile_offset(r, j), data + (at >= 0 ? at + j * 16 : 0), at >= 0);
+                        }
                     }
                 }
                 copy_commit();
@@ -337,21 +372,42 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                     __syncwarp();
                     if (lane == 0) {
                         if (c == kLag) barrier_arrive(q_full);
-                        barrier_arrive(full((c - kLag) % T::kSlots));
+                        if (!by_engine(c - kLag)) barrier_arrive(full((c - kLag) % T::kSlots));
                     }
                 }
             }
         } else {
             constexpr int kRowPieces = HD / 16, kRawRows = 32 / kRowPieces;
             auto fetch = [&](int c) {                                   // codes and scales of tile c into the ring of bytes
-                if (c < count) {
-                    if (c % 2 == 0) look_up(c / 2);
-                    const uint32_t to = base + T::kRaw + c % T::kRawSlots * T::kRawSlot;
+                if (c < count && ok) {
+                    const int slot = c % T::kRawSlots;
+                    const uint32_t to = base + T::kRaw + slot * T::kRawSlot;
                     const char* data = c % 2 ? v_data : k_data;
+                    if (by_engine(c)) {
+                        if (w > 0) return;
+                        if (c >= T::kRawSlots && !(ok = warp_wait(raw_empty + slot * 8, (c / T::kRawSlots - 1) & 1))) return;
+                        const int b = lane >> 1, first = range.begin + c / 2 * kTileKeys + b * p.box;
+                        int id = -1;
+                        if (b < boxes) id = block_of(p.batch, p.cache, seq, first);
+                        const bool there = b < boxes && id >= 0;
+                        bad |= b < boxes && id < 0;
+                        const int copies = __popc(__ballot_sync(0xffffffffu, there)) / 2;
+                        if (lane == 0) barrier_expect(raw_full + slot * 8, copies * p.box * (HD + 4));
+                        __syncwarp();
+                        if (there) {
+                            const char* tile_at = data + id * p.cache.block_stride + (int64_t)kv_head * p.cache.head_stride;
+                            const int offset = first % p.cache.block_size;
+                            if (lane & 1)
+                                bulk_copy(to + kTileKeys * HD + b * p.box * 4, tile_at + (int64_t)p.cache.block_size * HD + offset * 4, p.box * 4, raw_full + slot * 8);
+                            else
+                                bulk_copy(to + b * p.box * HD, tile_at + (int64_t)offset * HD, p.box * HD, raw_full + slot * 8);
+                        }
+                        return;
+                    }
+                    look_up(c / 2);
                     for (int g = w; g < kTileKeys / kRawRows; g += kLoadWarps) {
                         const int r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
-                        const int64_t mine = g * kRawRows < 32 ? at_k[0] : g * kRawRows < 64 ? at_k[1] : g * kRawRows < 96 ? at_k[2] : at_k[3];
-                        const int64_t packed = __shfl_sync(0xffffffffu, mine, r & 31);
+                        const int64_t packed = __shfl_sync(0xffffffffu, of_row(g * kRawRows, false), r & 31);
                         const int64_t tile_at = packed & 0xffffffffffll;
                         const int offset = (int)(packed >> 40);
                         const bool there = packed >= 0;
@@ -359,18 +415,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                         if (j == 0) copy4(to + kTileKeys * HD + r * 4, data + (there ? tile_at + (int64_t)p.cache.block_size * HD + offset * 4 : 0), there);
                     }
                 }
-                copy_commit();
             };
             fetch(0);
+            copy_commit();
             fetch(1);
-            for (int c = 0; c < count; ++c) {
+            copy_commit();
+            for (int c = 0; c < count && ok; ++c) {
                 fetch(c + 2);
+                copy_commit();
                 copy_wait<2>();
                 __syncwarp();
-                const int slot = c % T::kSlots;
+                const int slot = c % T::kSlots, raw_slot = c % T::kRawSlots;
+                if (!ok || (by_engine(c) && !(ok = warp_wait(raw_full + raw_slot * 8, c / T::kRawSlots & 1)))) break;
                 if (c >= T::kSlots && !(ok = warp_wait(empty(slot), (c / T::kSlots - 1) & 1))) break;
-                const unsigned char* raw = smem + T::kRaw + c % T::kRawSlots * T::kRawSlot;
+                const unsigned char* raw = smem + T::kRaw + raw_slot * T::kRawSlot;
                 unsigned char* to = smem + T::kRing + slot * T::kSlot;
+#pragma unroll 4
                 for (int g = w; g < kTileKeys / kRawRows; g += kLoadWarps) {
                     const int r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
                     uint4 lo, hi;
@@ -383,6 +443,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                 __syncwarp();
                 if (lane == 0) {
                     if (c == 0) barrier_arrive(q_full);                 // Q's copies are older than the first tile's
+                    barrier_arrive(raw_empty + raw_slot * 8);
                     barrier_arrive(full(slot));
                 }
             }

@@ -51,6 +51,26 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
 // Makes this thread's writes to shared memory visible to the tensor core and the copy engine.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// ---- copy engine: to shared memory, completing on a barrier ------------------------------------------------
+
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Addresses and sizes are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_copy(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+// A box of a tensor; x * element size is a multiple of 16 bytes.
+__device__ __forceinline__ void box_copy(uint32_t to, const void* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void box_copy(uint32_t to, const void* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+
 // ---- tensor memory ---------------------------------------------------------------------------------------
 
 // One warp allocates; the address is left in shared memory.
