@@ -78,9 +78,9 @@ EncodeTiled encode_tiled() {
     return f;
 }
 
-// Rows of 16-bit values in boxes of 64 values by `box` rows, 128-byte swizzle.  dims: values, [heads,] rows.
-bool encode_map(CUtensorMap* map, const void* data, int rank, const cuuint64_t* dims, const cuuint64_t* strides, int box, bool bf16) {
-    const cuuint32_t boxes[3] = {64, rank == 3 ? 1u : (cuuint32_t)box, (cuuint32_t)box}, steps[3] = {1, 1, 1};
+// Rows of 16-bit values in boxes of 64 values by [`heads` by] `box` rows, 128-byte swizzle.  dims: values, [heads,] rows.
+bool encode_map(CUtensorMap* map, const void* data, int rank, const cuuint64_t* dims, const cuuint64_t* strides, int box, bool bf16, int heads = 1) {
+    const cuuint32_t boxes[3] = {64, rank == 3 ? (cuuint32_t)heads : (cuuint32_t)box, (cuuint32_t)box}, steps[3] = {1, 1, 1};
     return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(data), dims,
                           strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -89,17 +89,24 @@ bool encode_map(CUtensorMap* map, const void* data, int rank, const cuuint64_t* 
 // Maps for this call, or p.box = 0 where the copy engine cannot follow the layout: blocks must tile 128 keys in
 // pieces of whole 1024-byte swizzle groups (8 rows).
 void make_maps(AttnParams& p, AttnMaps& maps, bool paged, bool e4m3, int64_t head_dim, bool bf16) {
-    p.box = 0;
+    p.box = p.q_box = 0;
+    const cuuint64_t num_rows = p.batch.num_rows;
+    auto strides = [&](const AttnRows& r, int64_t heads, cuuint64_t (&s)[2]) {       // the stride of a dimension of one says nothing
+        s[0] = heads > 1 ? r.head_stride : head_dim * 2;
+        s[1] = num_rows > 1 ? r.row_stride : head_dim * 2;
+    };
+    if (encode_tiled() && kTileRows % p.group == 0) {
+        const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)p.heads, num_rows};
+        cuuint64_t qs[2];
+        strides(p.q, p.heads, qs);
+        p.q_box = encode_map(&maps.q, p.q.data, 3, dims, qs, kTileRows / p.group, bf16, p.group);
+    }
     if (!paged) {
         if (!encode_tiled()) return;
-        const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)(p.heads / p.group), (cuuint64_t)p.batch.num_rows};
-        auto strides = [&](const AttnRows& r, cuuint64_t (&s)[2]) {       // the stride of a dimension of one says nothing
-            s[0] = dims[1] > 1 ? r.head_stride : head_dim * 2;
-            s[1] = dims[2] > 1 ? r.row_stride : head_dim * 2;
-        };
+        const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)(p.heads / p.group), num_rows};
         cuuint64_t ks[2], vs[2];
-        strides(p.k, ks);
-        strides(p.v, vs);
+        strides(p.k, p.heads / p.group, ks);
+        strides(p.v, p.heads / p.group, vs);
         if (encode_map(&maps.k, p.k.data, 3, dims, ks, kTileKeys, bf16) && encode_map(&maps.v, p.v.data, 3, dims, vs, kTileKeys, bf16)) p.box = kTileKeys;
         return;
     }
@@ -113,8 +120,8 @@ void make_maps(AttnParams& p, AttnMaps& maps, bool paged, bool e4m3, int64_t hea
     const int64_t rows = (int64_t)p.cache.num_blocks * p.layers * kv_heads * bs;
     if (!encode_tiled() || rows > INT32_MAX) return;
     const int64_t back = (int64_t)p.layer * kv_heads * p.cache.head_stride;          // from this layer to the pool's start
-    const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)head_dim * 2};
-    if (encode_map(&maps.k, p.cache.k - back, 2, dims, strides, box, bf16) && encode_map(&maps.v, p.cache.v - back, 2, dims, strides, box, bf16)) p.box = box;
+    const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows}, pitch[1] = {(cuuint64_t)head_dim * 2};
+    if (encode_map(&maps.k, p.cache.k - back, 2, dims, pitch, box, bf16) && encode_map(&maps.v, p.cache.v - back, 2, dims, pitch, box, bf16)) p.box = box;
 }
 
 template <int HD, bool BF16, bool PAGED, bool E4M3>

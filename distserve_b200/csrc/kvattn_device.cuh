@@ -22,12 +22,13 @@ struct AttnParams {
     float* part_out;                   // [row][head][split][head_dim], sums before the division
     float2* part_stat;                 // [row][head][split]: running maximum (base 2) and sum
     int32_t box;                       // keys that the copy engine moves at once; 0: it cannot follow this layout
+    int32_t q_box;                     // the same for Q: 1 if a tile of 128 rows is one box of tokens x query heads
     int32_t layers, layer;
 };
 
 // Maps of K and V for the copy engine: rows of head_dim values, copied in boxes of 64 values by up to 128 rows.
 struct AttnMaps {
-    CUtensorMap k, v;
+    CUtensorMap k, v, q;
 };
 
 // Keys of one sequence that split s reads: whole units of kSplitKeys, dealt evenly; later splits may have none.
@@ -97,6 +98,54 @@ __device__ __forceinline__ uint32_t widen2(uint32_t codes) {
     if (!BF16) return w;
     const float2 f = Half<false>::to_float2(w);
     return Half<true>::from_float2(f.x, f.y);
+}
+
+// Pairs of 32-bit floats: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    return x;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(x));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t x;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
+    return x;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t x;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+    return x;
+}
+
+// The larger of three, NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float x;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(x) : "f"(a), "f"(b), "f"(c));
+    return x;
+}
+
+// 2^x of two values on the multiply-add pipes instead of the special function unit, for x <= 126: 2^n 2^f with n the
+// nearest integer, and 2^f for |f| <= 1/2 by a polynomial of degree 4 fitted to the least relative error (2.7e-6,
+// a hundredth of a step of the 16-bit types that the result is rounded to).  Below 2^-126 the result stays at 2^-126.
+__device__ __forceinline__ float2 exp2_pair(uint64_t x) {
+    const float kMagic = 12582912.f;                      // 1.5 * 2^23: adding it leaves the integer in the low bits
+    float2 v = unpair(x);
+    v.x = fmaxf(v.x, -126.f);
+    v.y = fmaxf(v.y, -126.f);
+    x = pair(v.x, v.y);
+    const uint64_t t = add_pair(x, pair(kMagic, kMagic));
+    const uint64_t f = fma_pair(add_pair(t, pair(-kMagic, -kMagic)), pair(-1.f, -1.f), x);
+    uint64_t y = fma_pair(pair(0.009570102207362652f, 0.009570102207362652f), f, pair(0.05591786280274391f, 0.05591786280274391f));
+    y = fma_pair(y, f, pair(0.240247443318367f, 0.240247443318367f));
+    y = fma_pair(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
+    y = fma_pair(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
+    const float2 n = unpair(t), r = unpair(y);
+    return make_float2(__int_as_float((__float_as_int(n.x) << 23) + __float_as_int(r.x)), __int_as_float((__float_as_int(n.y) << 23) + __float_as_int(r.y)));
 }
 
 __device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fffffffu); }

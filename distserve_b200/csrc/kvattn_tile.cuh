@@ -30,7 +30,7 @@ template <int HD, bool E4M3> struct TileShape {
     static constexpr int kSlots = E4M3 ? 3 : 5;
     static constexpr int kRawSlot = E4M3 ? kTileKeys * (HD + 4) : 0;        // codes, then scales
     static constexpr int kRawSlots = E4M3 ? 3 : 0;
-    static constexpr int kBarriers = 2 * kSlots + 1 + 6 + 1 + 2 * kRawSlots;
+    static constexpr int kBarriers = 2 * kSlots + 1 + 8 + 1 + 2 * kRawSlots;
     static constexpr int kRing = 2 * kSlot, kRaw = kRing + kSlots * kSlot, kBars = kRaw + kRawSlots * kRawSlot;
     static constexpr int kShared = kBars + kBarriers * 8 + 32 + 1024;       // and room to align the start to 1024
 };
@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
     const uint32_t bars = base + T::kBars;
     auto full = [&](int s) { return bars + s * 8; };
     auto empty = [&](int s) { return bars + (T::kSlots + s) * 8; };
-    const uint32_t q_full = bars + 2 * T::kSlots * 8, s_full = q_full + 8, p_full = s_full + 16, pv_done = p_full + 16, drained = pv_done + 16, raw_full = drained + 8, raw_empty = raw_full + T::kRawSlots * 8;
+    const uint32_t q_full = bars + 2 * T::kSlots * 8, s_full = q_full + 8, p_half = s_full + 16, p_full = p_half + 16, pv_done = p_full + 16,
+                   drained = pv_done + 16, raw_full = drained + 8, raw_empty = raw_full + T::kRawSlots * 8;
     volatile int* flags = reinterpret_cast<volatile int*>(smem + T::kBars + T::kBarriers * 8);    // failed, bad, tensor memory
 
     // Which rows and keys.  Later row tiles, which have more keys, come first.
@@ -110,11 +111,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
     const KeyRange range = split_range(len, p.splits, split);
     const bool whole = split_range(len, p.splits, 0).end == len;
     if (split > 0 && (whole || range.begin >= len)) return;
+    // Row r of the block is token token0 + (skip + r) / group, query head (skip + r) % group of the group.
+    const int token0 = (int)(row0 / p.group), here = (int)min((int64_t)kBlockRows, total - row0);
+    const unsigned group = p.group, skip = (unsigned)(row0 - (int64_t)token0 * group);
     int n[2];                                          // key tiles of each row tile
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const int64_t end = min(row0 + (t + 1) * kTileRows, total);
-        const int keys = end <= row0 + t * kTileRows ? 0 : (int)min((int64_t)range.end, first_pos + (end - 1) / p.group + 1) - range.begin;
+        const int end = min((t + 1) * kTileRows, here);
+        const int keys = end <= t * kTileRows ? 0 : (int)min((int64_t)range.end, (int64_t)first_pos + token0 + (skip + end - 1) / group + 1) - range.begin;
         n[t] = keys > 0 ? (keys + kTileKeys - 1) / kTileKeys : 0;
     }
     const int steps = max(n[0], n[1]);
@@ -133,6 +137,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
         }
         for (int t = 0; t < 2; ++t) {
             barrier_init(s_full + t * 8, 1);
+            barrier_init(p_half + t * 8, 4);
             barrier_init(p_full + t * 8, 4);
             barrier_init(pv_done + t * 8, 1);
         }
@@ -145,21 +150,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = flags[2];
+    const uint32_t tmem = __shfl_sync(0xffffffffu, flags[2], 0);
     // A whole warp waits, and goes on or gives up together.
     auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(bar, parity, flags)) != 0; };
     // The sign of the scale is taken by the products and a scale of zero by Q, so that the maximum of the scores is theirs too.
     const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
 
     if (warp < kSoftmaxThreads / 32) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ---- softmax: a thread per row -------------------------------------------------------------------
         const int t = warp >> 2;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;             // this warp's 32 rows of tensor memory
         const uint32_t s_at = tmem + t * kTileKeys + lanes, o_at = tmem + 2 * kTileKeys + t * 128 + lanes;
-        const int64_t row = row0 + threadIdx.x;
-        const bool there = row < total;
-        const int64_t token = there ? row / p.group : 0;
-        const int last = there ? (int)min(first_pos + token, (int64_t)range.end - 1) : -1;      // last key that the row sees
+        const bool there = (int)threadIdx.x < here;
+        const int token = token0 + (skip + threadIdx.x) / group;
+        const int last = there ? (int)min((int64_t)first_pos + token, (int64_t)range.end - 1) : -1;      // last key that the row sees
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int i = 0; i < n[t]; ++i) {
@@ -167,40 +172,64 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
             tmem_fence_after();
             const int seen = last - (range.begin + i * kTileKeys);      // columns up to this one count
             const bool masked = __any_sync(0xffffffffu, seen < kTileKeys - 1);
-            uint32_t b[64];
-            float top = -INFINITY;
-            {
-                uint32_t a[64];
-                tmem_load(a, s_at);
-                if (masked)
+            uint32_t a[64], b[64];
+            tmem_load_async(a, s_at);
+            tmem_load_async(b, s_at + 64);
+            tmem_wait(a);
+            tmem_wait(b);
+            if (masked) {
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) a[j] = j <= seen ? a[j] : 0xff800000u;
-                float top2 = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 64; j += 2) {
-                    top = fmaxf(top, __uint_as_float(a[j]));
-                    top2 = fmaxf(top2, __uint_as_float(a[j + 1]));
+                for (int j = 0; j < 64; ++j) {
+                    a[j] = j <= seen ? a[j] : 0xff800000u;
+                    b[j] = j + 64 <= seen ? b[j] : 0xff800000u;
                 }
-                tmem_load(b, s_at + 64);
-                if (masked)
-#pragma unroll
-                    for (int j = 0; j < 64; ++j) b[j] = j + 64 <= seen ? b[j] : 0xff800000u;
-#pragma unroll
-                for (int j = 0; j < 64; j += 2) {
-                    top = fmaxf(top, __uint_as_float(b[j]));
-                    top2 = fmaxf(top2, __uint_as_float(b[j + 1]));
-                }
-                top = fmaxf(top, top2) * scale;
             }
-            if (i == 0) {
-                m = top;
-            } else {
-                const bool grown = top > m + kLazy;
-                if (__any_sync(0xffffffffu, grown)) {
+            const uint64_t scale2 = pair(scale, scale);
+            uint64_t sum[2] = {0, 0};
+            // Probabilities of 64 keys into 32 registers, two to a register; one pair in four by multiply-adds.
+            auto probabilities = [&](const uint32_t (&x)[64], uint32_t (&w)[32], uint64_t shift2) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const uint64_t e = fma_pair(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), scale2, shift2);
+                    float2 y;
+                    if (j % 4 == 3) {
+                        y = exp2_pair(e);
+                    } else {
+                        y = unpair(e);
+                        y.x = exp2_fast(y.x);
+                        y.y = exp2_fast(y.y);
+                    }
+                    sum[j % 2] = add_pair(sum[j % 2], pair(y.x, y.y));
+                    w[j] = H::from_float2(y.x, y.y);
+                }
+            };
+            auto hand_over = [&](uint32_t at, const uint32_t (&w)[32], uint32_t bar) {
+                tmem_store(at, w);
+                tmem_wait_store();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(bar);
+            };
+            // The maximum; NaN if a score is, and then everything of this row becomes NaN.
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) {
+                tops[0] = max_nan(tops[0], __uint_as_float(a[j]), __uint_as_float(a[j + 1]));
+                tops[1] = max_nan(tops[1], __uint_as_float(a[j + 2]), __uint_as_float(a[j + 3]));
+                tops[2] = max_nan(tops[2], __uint_as_float(b[j]), __uint_as_float(b[j + 1]));
+                tops[3] = max_nan(tops[3], __uint_as_float(b[j + 2]), __uint_as_float(b[j + 3]));
+            }
+            uint32_t w[32];
+            // All steps but the first begin with the maximum so far, as if this tile did not raise it beyond the allowance.
+            uint64_t shift2 = pair(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
+            if (i > 0) probabilities(a, w, shift2);
+            const float top = max_nan(max_nan(tops[0], tops[1], tops[2]), tops[3], -INFINITY) * scale;
+            const bool grown = i == 0 || !(top <= m + kLazy);
+            if (__any_sync(0xffffffffu, grown)) {
+                if (i > 0) {
                     if (!(ok = warp_wait(pv_done + t * 8, (i - 1) & 1))) break;
                     tmem_fence_after();
                     const float keep = grown ? exp2_fast(m - top) : 1.f;
-                    if (grown) m = top;
                     l *= keep;
 #pragma unroll
                     for (int j = 0; j < HD; j += 32) {
@@ -211,46 +240,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                         tmem_store(o_at + j, o);
                     }
                 }
+                if (grown) m = top;
+                shift2 = pair(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
+                sum[0] = sum[1] = 0;
+                probabilities(a, w, shift2);
             }
-            const float shift = m == -INFINITY ? 0.f : -m;
-            float sum[4] = {};
-            // Probabilities go where the second half of the scores was: columns 64 .. 127 of S, two to a column.
-            uint32_t w[32];
-#pragma unroll
-            for (int j = 0; j < 64; j += 2) {
-                const float x = exp2_fast(fmaf(__uint_as_float(b[j]), scale, shift));
-                const float y = exp2_fast(fmaf(__uint_as_float(b[j + 1]), scale, shift));
-                sum[j % 4] += x;
-                sum[j % 4 + 1] += y;
-                w[j / 2] = H::from_float2(x, y);
-            }
-            tmem_store(s_at + 96, w);
-            tmem_load(b, s_at);
-            if (masked)
-#pragma unroll
-                for (int j = 0; j < 64; ++j) b[j] = j <= seen ? b[j] : 0xff800000u;
-#pragma unroll
-            for (int j = 0; j < 64; j += 2) {
-                const float x = exp2_fast(fmaf(__uint_as_float(b[j]), scale, shift));
-                const float y = exp2_fast(fmaf(__uint_as_float(b[j + 1]), scale, shift));
-                sum[j % 4] += x;
-                sum[j % 4 + 1] += y;
-                w[j / 2] = H::from_float2(x, y);
-            }
-            tmem_store(s_at + 64, w);
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_wait_store();
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(p_full + t * 8);
+            hand_over(s_at + 64, w, p_half + t * 8);
+            probabilities(b, w, shift2);
+            hand_over(s_at + 96, w, p_full + t * 8);
+            const float2 parts = unpair(add_pair(sum[0], sum[1]));
+            l += parts.x + parts.y;
         }
         __syncwarp();
         asm volatile("bar.sync 1, 352;" ::: "memory");                  // the loading warps have said what they found
         if (ok && n[t] > 0) ok = warp_wait(pv_done + t * 8, (n[t] - 1) & 1);
         tmem_fence_after();
+        if (m == -INFINITY) l = 0.f;                                     // no key: zeros
         if (!ok || flags[0] || flags[1]) l = not_a_number();
         const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
-        const int64_t out_row = s.first + token, head = kv_head * p.group + (there ? row % p.group : 0);
+        const int64_t out_row = s.first + token, head = kv_head * group + (skip + threadIdx.x) % group;
         const int64_t part = (out_row * p.heads + head) * p.splits + split;
         char* to = p.out.data + out_row * p.out.row_stride + head * p.out.head_stride;
         if (there && !whole) p.part_stat[part] = make_float2(m, l);
@@ -280,17 +288,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
             }
         }
         tmem_fence_before();
-    } else if (warp < kSoftmaxThreads / 32 + kLoadWarps) {
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      if (warp < kSoftmaxThreads / 32 + kLoadWarps) {
         // ---- loading -------------------------------------------------------------------------------------
+        if (!E4M3 && p.box > 0 && lane == 0) {
+            prefetch_map(&maps.k);
+            prefetch_map(&maps.v);
+        }
         const int w = warp - kSoftmaxThreads / 32;
         constexpr int kRowsAtOnce = 32 / kPieces;                       // rows that a warp copies with one instruction
-        for (int g = w; g < kBlockRows / kRowsAtOnce; g += kLoadWarps) {
-            const int r = g * kRowsAtOnce + lane / kPieces, j = lane % kPieces;
-            const int64_t row = row0 + r;
-            const bool there = row < total && p.scale_log2 != 0.f;
-            const char* from = p.q.data;
-            if (there) from += (s.first + row / p.group) * p.q.row_stride + (kv_head * p.group + row % p.group) * p.q.head_stride + j * 16;
-            copy16(base + (r / kTileRows) * T::kSlot + tile_offset(r % kTileRows, j), from, there);
+        const bool q_by_engine = p.q_box > 0 && p.scale_log2 != 0.f;
+        if (q_by_engine) {
+            // 128 rows are 128 / group tokens of all the group's heads, and row0 is the first head of one.
+            if (w == 0 && lane == 0 && steps > 0) {
+                barrier_expect(q_full, 2 * T::kSlot);
+                for (int t = 0; t < 2; ++t)
+                    for (int h = 0; h < HD / 64; ++h)
+                        box_copy(base + t * T::kSlot + h * kTileRows * 128, &maps.q, h * 64, kv_head * (int)group, s.first + token0 + t * (kTileRows / (int)group), q_full);
+            }
+        } else {
+            for (int x = 0; x < kBlockRows; x += 32) {                  // each lane finds the place of one row of 32
+                const int mine = x + lane;
+                const bool there = mine < here && p.scale_log2 != 0.f;
+                const unsigned token = (skip + mine) / group, head = (skip + mine) % group;
+                const int64_t at = there ? (int64_t)(s.first + token0 + token) * p.q.row_stride + (int64_t)(kv_head * group + head) * p.q.head_stride : -1;
+                for (int g = w; g < 32 / kRowsAtOnce; g += kLoadWarps) {
+                    const int r = g * kRowsAtOnce + lane / kPieces, j = lane % kPieces;
+                    const int64_t from = __shfl_sync(0xffffffffu, at, r);
+                    copy16(base + (x / kTileRows) * T::kSlot + tile_offset(x % kTileRows + r, j), p.q.data + (from >= 0 ? from + j * 16 : 0), from >= 0);
+                }
+            }
         }
         copy_commit();
         const int count = 2 * steps;                                    // K and V tiles in turn
@@ -326,7 +354,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
         const char* k_data = PAGED ? p.cache.k : p.k.data;
         const char* v_data = PAGED ? p.cache.v : p.v.data;
         constexpr int kLag = 2;                                         // tiles in flight behind the newest
-        if (!E4M3) {
+        if constexpr (!E4M3) {
             for (int c = 0; c < count + kLag; ++c) {
                 if (c < count) {
                     const int slot = c % T::kSlots;
@@ -371,7 +399,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                     fence_async_shared();
                     __syncwarp();
                     if (lane == 0) {
-                        if (c == kLag) barrier_arrive(q_full);
+                        if (c == kLag && !(q_by_engine && w == 0)) barrier_arrive(q_full);
                         if (!by_engine(c - kLag)) barrier_arrive(full((c - kLag) % T::kSlots));
                     }
                 }
@@ -442,7 +470,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                 fence_async_shared();
                 __syncwarp();
                 if (lane == 0) {
-                    if (c == 0) barrier_arrive(q_full);                 // Q's copies are older than the first tile's
+                    if (c == 0 && !(q_by_engine && w == 0)) barrier_arrive(q_full);      // Q's copies are older than the first tile's
                     barrier_arrive(raw_empty + raw_slot * 8);
                     barrier_arrive(full(slot));
                 }
@@ -454,64 +482,89 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
         __syncwarp();
         asm volatile("bar.arrive 1, 352;" ::: "memory");
     } else {
-        // ---- products: one thread issues them all ---------------------------------------------------------
-        if (lane == 0 && steps > 0) {
+        // ---- products: one lane issues them all -----------------------------------------------------------
+        if (steps > 0) {
             const uint32_t s_kind = product_kind(BF16, kTileRows, kTileKeys, false, false) | (p.scale_log2 < 0.f ? 1u << 13 : 0u);
             constexpr uint32_t o_kind = product_kind(BF16, kTileRows, HD, true, false);
-            bool ok = barrier_wait(q_full, 0, flags);
+            const bool leader = elect_one();
+            const uint64_t q_desc = operand(base, 16, 1024), k_desc = operand(base + T::kRing, 16, 1024),
+                           v_desc = operand(base + T::kRing, kTileKeys * 128, 1024);
+            bool ok = warp_wait(q_full, 0);
             auto scores = [&](int t, int slot) {
-                const uint32_t k_at = base + T::kRing + slot * T::kSlot, q_at = base + t * T::kSlot;
+                const uint64_t a = q_desc + t * (T::kSlot >> 4), b = k_desc + slot * (T::kSlot >> 4);
+                if (leader) {
 #pragma unroll
-                for (int x = 0; x < HD / 16; ++x) {
-                    const uint32_t step = (x / 4) * (kTileKeys * 128) + (x % 4) * 32;
-                    mma_shared(tmem + t * kTileKeys, operand(q_at + step, 16, 1024), operand(k_at + step, 16, 1024), s_kind, x > 0);
+                    for (int x = 0; x < HD / 16; ++x) {
+                        const uint32_t step = ((x / 4) * (kTileKeys * 128) + (x % 4) * 32) >> 4;
+                        mma_shared(tmem + t * kTileKeys, a + step, b + step, s_kind, x > 0);
+                    }
+                    mma_commit(s_full + t * 8);
                 }
-                mma_commit(s_full + t * 8);
+                __syncwarp();
             };
-            if (ok) ok = barrier_wait(full(0), 0, flags);
+            auto outputs = [&](int t, int slot, int half, bool add) {   // 64 keys
+                const uint64_t b = v_desc + slot * (T::kSlot >> 4);
+                if (leader) {
+#pragma unroll
+                    for (int y = 0; y < kTileKeys / 32; ++y) {
+                        const int x = half * (kTileKeys / 32) + y;
+                        mma_tmem(tmem + 2 * kTileKeys + t * 128, tmem + t * kTileKeys + 64 + x * 8, b + x * (2048 >> 4), o_kind, add || y > 0);
+                    }
+                    if (half) mma_commit(pv_done + t * 8);
+                }
+                __syncwarp();
+            };
+            auto release = [&](int slot) {
+                if (leader) mma_commit(empty(slot));
+                __syncwarp();
+            };
+            if (ok) ok = warp_wait(full(0), 0);
             if (ok) {
                 tmem_fence_after();
-                for (int t = 0; t < 2; ++t)
-                    if (n[t] > 0) scores(t, 0);
-                mma_commit(empty(0));
+                if (n[0] > 0) scores(0, 0);
+                if (n[1] > 0) scores(1, 0);
+                release(0);
             }
+            int slot = 0, phase = 0;                                    // of the tile that was last waited for
             for (int i = 0; i < steps && ok; ++i) {
-                const int v = 2 * i + 1, k = 2 * i + 2, v_slot = v % T::kSlots, k_slot = k % T::kSlots;
-                ok = barrier_wait(full(v_slot), (v / T::kSlots) & 1, flags);
+                auto next = [&](int& at, int& ph) { if (++at == T::kSlots) { at = 0; ph ^= 1; } };
+                next(slot, phase);
+                const int v_slot = slot;
+                if (!(ok = warp_wait(full(v_slot), phase))) break;
+                const bool more = i + 1 < steps;
+                if (more) next(slot, phase);
                 bool k_ready = false;
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (i >= n[t]) continue;
-                    if (!(ok = barrier_wait(p_full + t * 8, i & 1, flags))) break;
-                    tmem_fence_after();
-                    const uint32_t v_at = base + T::kRing + v_slot * T::kSlot;
 #pragma unroll
-                    for (int x = 0; x < kTileKeys / 16; ++x)
-                        mma_tmem(tmem + 2 * kTileKeys + t * 128, tmem + t * kTileKeys + 64 + x * 8, operand(v_at + x * 2048, kTileKeys * 128, 1024),
-                                 o_kind, i > 0 || x > 0);
-                    mma_commit(pv_done + t * 8);
-                    if (i + 1 < n[t]) {
-                        if (!k_ready) {
-                            if (!(ok = barrier_wait(full(k_slot), (k / T::kSlots) & 1, flags))) break;
-                            tmem_fence_after();
-                            k_ready = true;
-                        }
-                        scores(t, k_slot);
+                for (int t = 0; t < 2; ++t) {
+                    if (i >= n[t] || !ok) continue;
+                    if (!(ok = warp_wait(p_half + t * 8, i & 1))) continue;
+                    tmem_fence_after();
+                    outputs(t, v_slot, 0, i > 0);
+                    if (i + 1 < n[t] && !k_ready) {
+                        if (!(ok = warp_wait(full(slot), phase))) continue;
+                        k_ready = true;
                     }
+                    if (!(ok = warp_wait(p_full + t * 8, i & 1))) continue;
+                    tmem_fence_after();
+                    outputs(t, v_slot, 1, true);
+                    if (i + 1 < n[t]) scores(t, slot);
                 }
-                if (ok) {
-                    mma_commit(empty(v_slot));
-                    if (k_ready) mma_commit(empty(k_slot));
-                }
+                if (!ok) break;
+                release(v_slot);
+                if (more) release(slot);
             }
             if (!ok) {
                 // products still in flight read shared memory and write tensor memory: give them their chance to end
-                atomicAdd(&g_attention_timeouts, 1u);
-                mma_commit(drained);
+                if (leader) {
+                    atomicAdd(&g_attention_timeouts, 1u);
+                    mma_commit(drained);
+                }
                 int quiet = 0;
                 barrier_wait(drained, 0, &quiet);
             }
         }
         __syncwarp();
+      }
     }
     __syncthreads();
     if (warp == kTileThreads / 32 - 1) {

@@ -30,7 +30,7 @@ constexpr unsigned kWaitPolls = 1u << 26;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 // Waits for a phase, for two seconds at most or until another thread of the block has given up (*failed).
-static __device__ __noinline__ bool barrier_wait_slow(uint32_t bar, uint32_t parity, volatile int* failed) {
+__device__ __forceinline__ bool barrier_wait_slow(uint32_t bar, uint32_t parity, volatile int* failed) {
     unsigned long long t0, t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
     for (unsigned i = 0; i < kWaitPolls; ++i) {
@@ -61,6 +61,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, const void* from, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const void* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // A box of a tensor; x * element size is a multiple of 16 bytes.
 __device__ __forceinline__ void box_copy(uint32_t to, const void* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -86,29 +87,41 @@ __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define KVMIG_R8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), "=r"(x[i + 6]), "=r"(x[i + 7])
+#define KVMIG_X8(x, i) "+r"(x[i]), "+r"(x[i + 1]), "+r"(x[i + 2]), "+r"(x[i + 3]), "+r"(x[i + 4]), "+r"(x[i + 5]), "+r"(x[i + 6]), "+r"(x[i + 7])
 #define KVMIG_W8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]), "r"(x[i + 7])
 
-// 32 or 64 columns of the lane's row; the values are there when this returns.
+// 32 columns of the lane's row; the values are there when this returns.
 __device__ __forceinline__ void tmem_load(uint32_t (&x)[32], uint32_t at) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
         "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
         : KVMIG_R8(x, 0), KVMIG_R8(x, 8), KVMIG_R8(x, 16), KVMIG_R8(x, 24) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void tmem_load(uint32_t (&x)[64], uint32_t at) {
+// 64 columns; the values are there after tmem_wait(x).
+__device__ __forceinline__ void tmem_load_async(uint32_t (&x)[64], uint32_t at) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
         "%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,"
-        "%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+        "%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
         : KVMIG_R8(x, 0), KVMIG_R8(x, 8), KVMIG_R8(x, 16), KVMIG_R8(x, 24), KVMIG_R8(x, 32), KVMIG_R8(x, 40), KVMIG_R8(x, 48), KVMIG_R8(x, 56)
         : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&x)[64]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : KVMIG_X8(x, 0), KVMIG_X8(x, 8), KVMIG_X8(x, 16), KVMIG_X8(x, 24), KVMIG_X8(x, 32), KVMIG_X8(x, 40), KVMIG_X8(x, 48), KVMIG_X8(x, 56)
+                 :: "memory");
 }
 __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&x)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
         "%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at), KVMIG_W8(x, 0), KVMIG_W8(x, 8), KVMIG_W8(x, 16), KVMIG_W8(x, 24) : "memory");
 }
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&x)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(at), KVMIG_W8(x, 0), KVMIG_W8(x, 8) : "memory");
+}
 #undef KVMIG_R8
+#undef KVMIG_X8
 #undef KVMIG_W8
 
 // ---- products --------------------------------------------------------------------------------------------
@@ -136,6 +149,13 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
+}
+// One lane of a converged warp, the same one every time.  What it issues sits in warp-uniform control flow, so that the
+// compiler can keep descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
 }
 // The barrier receives one arrival when everything that this thread has issued is done.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
