@@ -134,7 +134,7 @@ int launch_tiles(const AttnParams& params, cudaStream_t stream, const char* what
     const int64_t grid = std::max<int64_t>(tiles, 1) * (p.heads / p.group) * p.batch.num_seqs;
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attend_tiles<HD, BF16, PAGED, E4M3><<<dim3((unsigned)grid, p.splits), kTileThreads, smem, stream>>>(p, maps);
+    attend_tiles<HD, BF16, PAGED, E4M3><<<dim3((unsigned)grid, p.splits), TileShape<HD, E4M3>::kThreads, smem, stream>>>(p, maps);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
     return 0;

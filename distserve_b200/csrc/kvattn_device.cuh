@@ -129,25 +129,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     return x;
 }
 
-// 2^x of two values on the multiply-add pipes instead of the special function unit, for x <= 126: 2^n 2^f with n the
-// nearest integer, and 2^f for |f| <= 1/2 by a polynomial of degree 4 fitted to the least relative error (2.7e-6,
-// a hundredth of a step of the 16-bit types that the result is rounded to).  Below 2^-126 the result stays at 2^-126.
-__device__ __forceinline__ float2 exp2_pair(uint64_t x) {
-    const float kMagic = 12582912.f;                      // 1.5 * 2^23: adding it leaves the integer in the low bits
-    float2 v = unpair(x);
-    v.x = fmaxf(v.x, -126.f);
-    v.y = fmaxf(v.y, -126.f);
-    x = pair(v.x, v.y);
-    const uint64_t t = add_pair(x, pair(kMagic, kMagic));
-    const uint64_t f = fma_pair(add_pair(t, pair(-kMagic, -kMagic)), pair(-1.f, -1.f), x);
-    uint64_t y = fma_pair(pair(0.009570102207362652f, 0.009570102207362652f), f, pair(0.05591786280274391f, 0.05591786280274391f));
-    y = fma_pair(y, f, pair(0.240247443318367f, 0.240247443318367f));
-    y = fma_pair(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
-    y = fma_pair(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
-    const float2 n = unpair(t), r = unpair(y);
-    return make_float2(__int_as_float((__float_as_int(n.x) << 23) + __float_as_int(r.x)), __int_as_float((__float_as_int(n.y) << 23) + __float_as_int(r.y)));
-}
-
 __device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fffffffu); }
 
 }  // namespace kvmig

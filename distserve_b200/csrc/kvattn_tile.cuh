@@ -6,8 +6,7 @@
 //   P = 2^(scale S - m), rounded to 16 bits, written back over S's columns;
 //   O += P V    128 x head_dim x 128, P from tensor memory, sums in tensor memory.
 // Each tile has a warpgroup with a thread per row for the softmax, so no value crosses threads.  While one tile's
-// softmax runs the tensor core works on the other's products; one thread issues all of them.  The remaining three warps
-// fill a ring of K and V tiles in shared memory: whole tiles through the copy engine, a box per block and 64 values, and
+// XX a ring of K and V tiles in shared memory: whole tiles through the copy engine, a box per block and 64 values, and
 // what it cannot follow (a sequence's last keys, whose neighbours in the block must become zeros; block sizes that
 // do not tile 128 keys) with cp.async.  Quantised pools pass through a second ring of bytes and are widened to 16 bits
 // by those warps.
@@ -22,12 +21,15 @@
 namespace kvmig {
 
 constexpr int kTileRows = 128, kTileKeys = 128, kBlockRows = 2 * kTileRows;
-constexpr int kSoftmaxThreads = 256, kLoadWarps = 3, kTileThreads = kSoftmaxThreads + kLoadWarps * 32 + 32;
+constexpr int kSoftmaxThreads = 256;
 constexpr float kLazy = 8.f;                 // the maximum may lag behind by this many powers of two
 
 template <int HD, bool E4M3> struct TileShape {
     static constexpr int kSlot = kTileKeys * HD * 2;                        // a 16-bit tile of K, V or Q
     static constexpr int kSlots = E4M3 ? 3 : 5;
+    static constexpr int kLoadWarps = E4M3 ? 7 : 3, kThreads = kSoftmaxThreads + kLoadWarps * 32 + 32;
+    // Registers of a softmax thread and of the others: together what the block is launched with (168 or 128 a thread).
+    static constexpr int kSoftmaxRegisters = E4M3 ? 200 : 208, kOtherRegisters = E4M3 ? 56 : 88;
     static constexpr int kRawSlot = E4M3 ? kTileKeys * (HD + 4) : 0;        // codes, then scales
     static constexpr int kRawSlots = E4M3 ? 3 : 0;
     static constexpr int kBarriers = 2 * kSlots + 1 + 8 + 1 + 2 * kRawSlots;
@@ -74,10 +76,11 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int j) {
 __device__ unsigned int g_attention_timeouts;      // blocks that gave up waiting
 
 template <int HD, bool BF16, bool PAGED, bool E4M3>
-__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_constant__ AttnParams p, const __grid_constant__ AttnMaps maps) {
+__global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_tiles(const __grid_constant__ AttnParams p, const __grid_constant__ AttnMaps maps) {
     using T = TileShape<HD, E4M3>;
     using H = Half<BF16>;
     constexpr int kPieces = HD / 8;                    // 16-byte pieces of a 16-bit row
+    constexpr int kLoadWarps = T::kLoadWarps, kTileThreads = T::kThreads;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + (1024 - (shared_address(smem_raw) & 1023)) % 1024;
     const uint32_t base = shared_address(smem);
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
     const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
 
     if (warp < kSoftmaxThreads / 32) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftmaxRegisters));
         // ---- softmax: a thread per row -------------------------------------------------------------------
         const int t = warp >> 2;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;             // this warp's 32 rows of tensor memory
@@ -186,19 +189,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
             }
             const uint64_t scale2 = pair(scale, scale);
             uint64_t sum[2] = {0, 0};
-            // Probabilities of 64 keys into 32 registers, two to a register; one pair in four by multiply-adds.
-            auto probabilities = [&](const uint32_t (&x)[64], uint32_t (&w)[32], uint64_t shift2) {
+            // Probabilities of 64 keys into 32 registers, two to a register.
+            // The maximum; NaN if a score is, and then everything of this row becomes NaN.
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto probabilities = [&](const uint32_t (&x)[64], uint32_t (&w)[32], uint64_t shift2, bool find_top) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                    const uint64_t e = fma_pair(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), scale2, shift2);
-                    float2 y;
-                    if (j % 4 == 3) {
-                        y = exp2_pair(e);
-                    } else {
-                        y = unpair(e);
-                        y.x = exp2_fast(y.x);
-                        y.y = exp2_fast(y.y);
+                    if (find_top) {
+                        tops[j % 2] = max_nan(tops[j % 2], __uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1]));
+                        tops[j % 2 + 2] = max_nan(tops[j % 2 + 2], __uint_as_float(b[2 * j]), __uint_as_float(b[2 * j + 1]));
                     }
+                    const uint64_t e = fma_pair(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), scale2, shift2);
+                    float2 y = unpair(e);
+                    y.x = exp2_fast(y.x);
+                    y.y = exp2_fast(y.y);
                     sum[j % 2] = add_pair(sum[j % 2], pair(y.x, y.y));
                     w[j] = H::from_float2(y.x, y.y);
                 }
@@ -210,19 +214,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                 __syncwarp();
                 if (lane == 0) barrier_arrive(bar);
             };
-            // The maximum; NaN if a score is, and then everything of this row becomes NaN.
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                tops[0] = max_nan(tops[0], __uint_as_float(a[j]), __uint_as_float(a[j + 1]));
-                tops[1] = max_nan(tops[1], __uint_as_float(a[j + 2]), __uint_as_float(a[j + 3]));
-                tops[2] = max_nan(tops[2], __uint_as_float(b[j]), __uint_as_float(b[j + 1]));
-                tops[3] = max_nan(tops[3], __uint_as_float(b[j + 2]), __uint_as_float(b[j + 3]));
-            }
             uint32_t w[32];
-            // All steps but the first begin with the maximum so far, as if this tile did not raise it beyond the allowance.
+            // Every step begins with the maximum so far, as if this tile did not raise it beyond the allowance.
             uint64_t shift2 = pair(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
-            if (i > 0) probabilities(a, w, shift2);
+            probabilities(a, w, shift2, true);
             const float top = max_nan(max_nan(tops[0], tops[1], tops[2]), tops[3], -INFINITY) * scale;
             const bool grown = i == 0 || !(top <= m + kLazy);
             if (__any_sync(0xffffffffu, grown)) {
@@ -243,16 +238,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
                 if (grown) m = top;
                 shift2 = pair(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
                 sum[0] = sum[1] = 0;
-                probabilities(a, w, shift2);
+                probabilities(a, w, shift2, false);
             }
             hand_over(s_at + 64, w, p_half + t * 8);
-            probabilities(b, w, shift2);
+            probabilities(b, w, shift2, false);
             hand_over(s_at + 96, w, p_full + t * 8);
             const float2 parts = unpair(add_pair(sum[0], sum[1]));
             l += parts.x + parts.y;
         }
         __syncwarp();
-        asm volatile("bar.sync 1, 352;" ::: "memory");                  // the loading warps have said what they found
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads + kLoadWarps * 32) : "memory");                  // the loading warps have said what they found
         if (ok && n[t] > 0) ok = warp_wait(pv_done + t * 8, (n[t] - 1) & 1);
         tmem_fence_after();
         if (m == -INFINITY) l = 0.f;                                     // no key: zeros
@@ -289,7 +284,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
         }
         tmem_fence_before();
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegisters));
       if (warp < kSoftmaxThreads / 32 + kLoadWarps) {
         // ---- loading -------------------------------------------------------------------------------------
         if (!E4M3 && p.box > 0 && lane == 0) {
@@ -480,7 +475,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles(const __grid_con
         if (bad) flags[1] = 1;
         __threadfence_block();
         __syncwarp();
-        asm volatile("bar.arrive 1, 352;" ::: "memory");
+        asm volatile("bar.arrive 1, %0;" ::"n"(kSoftmaxThreads + kLoadWarps * 32) : "memory");
     } else {
         // ---- products: one lane issues them all -----------------------------------------------------------
         if (steps > 0) {
