@@ -14,36 +14,42 @@
 namespace kvmig {
 namespace {
 
-// Blocks that the device holds at once when two share an SM (B200: 148 SMs).
-constexpr int64_t kResident = 2 * 148;
+constexpr int64_t kSms = 148;      // of a B200
 
-// Up to 16 rows of a sequence share a KV head: the kernel for few rows.
-bool few_rows(int64_t max_rows, int64_t group) { return max_rows * group <= kFewRows; }
-
-// Parts that a sequence's keys are cut into: as many as fill the device, but none shorter than 256 keys of what the
-// block tables have room for.
-int64_t splits_for(int64_t tiles, int64_t capacity) {
-    const int64_t fill = kResident / std::max<int64_t>(tiles, 1), longest = std::max<int64_t>(capacity / 256, 1);
-    return std::max<int64_t>(1, std::min(std::min(fill, longest), (int64_t)256));
-}
-
+// How a paged call is run.  Sequences with up to kFewMost rows per KV head go to the kernel for few rows (all of them if
+// none can have more), the others to the tile kernel; one of the two is launched if the batch can be seen to need only
+// that one.
 struct PagedPlan {
-    bool few;
-    int64_t splits, workspace;
+    bool few, tiles;
+    int64_t few_rows, few_tile, parts, workspace;
+    SplitRule few_rule, tile_rule;
 };
 
 PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_batch* b) {
     PagedPlan plan = {};
-    plan.few = few_rows(b->max_rows, heads / shape->num_heads);
-    const int64_t capacity = std::min<int64_t>(b->max_blocks * shape->block_size, INT32_MAX);
-    if (plan.few) {
-        plan.splits = splits_for(b->num_seqs * shape->num_heads, capacity);
-    } else {
-        const int64_t tiles = (b->num_rows * (heads / shape->num_heads) / kBlockRows + b->num_seqs) * shape->num_heads;
-        plan.splits = splits_for(2 * tiles, capacity);        // a block has an SM to itself
-    }
-    const int64_t head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
-    if (plan.splits > 1) plan.workspace = b->num_rows * heads * plan.splits * (head_dim * 4 + (int64_t)sizeof(float2));
+    const int64_t group = heads / shape->num_heads, most = std::min(b->max_rows, b->num_rows) * group;
+    const int64_t capacity = std::min<int64_t>(b->max_blocks * shape->block_size, INT32_MAX), units = (capacity + kSplitKeys - 1) / kSplitKeys;
+    plan.tiles = most > kFewMost;
+    // rows for every sequence to have its most: as good as certain that all have many
+    plan.few = !plan.tiles || b->num_rows < b->num_seqs * b->max_rows;
+    plan.few_rows = !plan.tiles ? INT64_MAX : plan.few ? kFewMost : 0;
+    plan.few_tile = most <= 16 ? 16 : 32;
+    const int64_t kv_heads = shape->num_heads, head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
+    // A part is at least the call's work over the blocks that the device holds at once (see part_units), so a sequence
+    // has no more parts than `fill`; the grid has a block for each, of which most return at once when there are many
+    // sequences, hence the bound by their number; and partial results stay below 256 MB.
+    const int64_t room = std::max<int64_t>((256 << 20) / std::max<int64_t>(b->num_rows * heads * (head_dim * 4 + 8), 1), 1);
+    auto rule = [&](int64_t blocks, int64_t least, int64_t most_blocks, int64_t tiles) {
+        const int64_t fill = blocks / kv_heads + 1, grid = most_blocks / std::max<int64_t>(b->num_seqs * kv_heads * tiles, 1);
+        const int64_t parts = std::min(std::min(units / least, fill), std::min(grid, room));
+        return SplitRule{(int32_t)std::max<int64_t>(parts, 1), (int32_t)least, (int32_t)blocks};
+    };
+    plan.few_rule = plan.tile_rule = SplitRule{1, 1, 1};
+    if (plan.few) plan.few_rule = rule(2 * kSms, 2, 4096, (std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile);
+    // A block of the tile kernel has an SM to itself; twice as many parts even out sequences of different lengths.
+    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, 16384, 1);
+    plan.parts = std::max(plan.few_rule.parts, plan.tile_rule.parts);
+    if (plan.parts > 1) plan.workspace = b->num_rows * heads * plan.parts * (head_dim * 4 + (int64_t)sizeof(float2));
     return plan;
 }
 
@@ -52,11 +58,14 @@ BatchView batch_view(const kvmig_batch* batch) {
                      (int32_t)batch->num_rows, (int32_t)batch->max_rows, (int32_t)batch->max_blocks};
 }
 
-template <int HD, bool BF16, bool E4M3>
-int launch_few(const AttnParams& p, unsigned grid, cudaStream_t stream) {
-    constexpr int smem = FewShape<HD, E4M3>::kShared;
-    CU_TRY(cudaFuncSetAttribute(attend_few<HD, BF16, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attend_few<HD, BF16, E4M3><<<dim3(grid, p.splits), kFewWarps * 32, smem, stream>>>(p);
+template <int HD, bool BF16, bool E4M3, int MT>
+int launch_few(const AttnParams& p, cudaStream_t stream, const char* what) {
+    constexpr int smem = FewShape<HD, E4M3, MT>::kShared, rows = FewShape<HD, E4M3, MT>::kRows;
+    const int64_t most = std::min((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group, (int64_t)kFewMost);
+    const int64_t grid = (int64_t)p.batch.num_seqs * (p.heads / p.group) * std::max<int64_t>((most + rows - 1) / rows, 1);
+    if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many sequences for one call", what);
+    CU_TRY(cudaFuncSetAttribute(attend_few<HD, BF16, E4M3, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attend_few<HD, BF16, E4M3, MT><<<dim3((unsigned)grid, p.few.parts), kFewWarps * 32, smem, stream>>>(p);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
     return 0;
@@ -125,7 +134,7 @@ void make_maps(AttnParams& p, AttnMaps& maps, bool paged, bool e4m3, int64_t hea
 }
 
 template <int HD, bool BF16, bool PAGED, bool E4M3>
-int launch_tiles(const AttnParams& params, cudaStream_t stream, const char* what) {
+int launch_tiles(const AttnParams& params, bool after_few, cudaStream_t stream, const char* what) {
     AttnParams p = params;
     AttnMaps maps = {};
     make_maps(p, maps, PAGED, E4M3, HD, BF16);
@@ -134,25 +143,30 @@ int launch_tiles(const AttnParams& params, cudaStream_t stream, const char* what
     const int64_t grid = std::max<int64_t>(tiles, 1) * (p.heads / p.group) * p.batch.num_seqs;
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attend_tiles<HD, BF16, PAGED, E4M3><<<dim3((unsigned)grid, p.splits), TileShape<HD, E4M3>::kThreads, smem, stream>>>(p, maps);
-    CU_TRY(cudaGetLastError());
+    // After the kernel for few rows, which has other rows to do: begins when that one's blocks leave room.
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)grid, p.tiles.parts);
+    config.blockDim = dim3(TileShape<HD, E4M3>::kThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = after_few ? 1 : 0;
+    CU_TRY(cudaLaunchKernelEx(&config, attend_tiles<HD, BF16, PAGED, E4M3>, p, maps));
     g_attention_launches++;
     return 0;
 }
 
-template <int HD, bool BF16>
-int launch(const AttnParams& p, bool paged, bool e4m3, bool few, cudaStream_t stream, const char* what) {
-    int rc;
-    if (few) {
-        const int64_t grid = (int64_t)p.batch.num_seqs * (p.heads / p.group);
-        if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many sequences for one call", what);
-        rc = e4m3 ? launch_few<HD, BF16, true>(p, (unsigned)grid, stream) : launch_few<HD, BF16, false>(p, (unsigned)grid, stream);
-    } else if (!paged) {
-        rc = launch_tiles<HD, BF16, false, false>(p, stream, what);
-    } else {
-        rc = e4m3 ? launch_tiles<HD, BF16, true, true>(p, stream, what) : launch_tiles<HD, BF16, true, false>(p, stream, what);
+template <int HD, bool BF16, bool E4M3>
+int launch_paged(const AttnParams& p, const PagedPlan& plan, cudaStream_t stream, const char* what) {
+    int rc = 0;
+    if (plan.few) {
+        rc = p.few_tile == 16 ? launch_few<HD, BF16, E4M3, 1>(p, stream, what) : launch_few<HD, BF16, E4M3, 2>(p, stream, what);
     }
-    if (rc || p.splits == 1) return rc;
+    if (!rc && plan.tiles) rc = launch_tiles<HD, BF16, true, E4M3>(p, plan.few, stream, what);
+    if (rc || p.parts == 1) return rc;
     const int64_t grid = ((int64_t)p.batch.num_rows * p.heads + 3) / 4;
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     attend_join<HD, BF16><<<(unsigned)grid, 128, 0, stream>>>(p);
@@ -161,15 +175,21 @@ int launch(const AttnParams& p, bool paged, bool e4m3, bool few, cudaStream_t st
     return 0;
 }
 
-int attend(AttnParams& p, bool paged, bool e4m3, bool few, int64_t head_dim, int dtype, const kvmig_batch* batch, cudaStream_t stream,
+template <int HD, bool BF16>
+int launch(const AttnParams& p, const PagedPlan* plan, bool e4m3, cudaStream_t stream, const char* what) {
+    if (!plan) return launch_tiles<HD, BF16, false, false>(p, false, stream, what);
+    return e4m3 ? launch_paged<HD, BF16, true>(p, *plan, stream, what) : launch_paged<HD, BF16, false>(p, *plan, stream, what);
+}
+
+int attend(AttnParams& p, const PagedPlan* plan, bool e4m3, int64_t head_dim, int dtype, const kvmig_batch* batch, cudaStream_t stream,
            const char* what) {
     p.batch = batch_view(batch);
     int dev;
     CU_TRY(cudaGetDevice(&dev));
     if (batch->num_rows == 0 || batch->num_seqs == 0) return 0;
     if (head_dim == 64)
-        return dtype == KVMIG_F16 ? launch<64, false>(p, paged, e4m3, few, stream, what) : launch<64, true>(p, paged, e4m3, few, stream, what);
-    return dtype == KVMIG_F16 ? launch<128, false>(p, paged, e4m3, few, stream, what) : launch<128, true>(p, paged, e4m3, few, stream, what);
+        return dtype == KVMIG_F16 ? launch<64, false>(p, plan, e4m3, stream, what) : launch<64, true>(p, plan, e4m3, stream, what);
+    return dtype == KVMIG_F16 ? launch<128, false>(p, plan, e4m3, stream, what) : launch<128, true>(p, plan, e4m3, stream, what);
 }
 
 AttnRows view(const kvmig_rows* r) { return AttnRows{static_cast<char*>(r->data), r->row_stride * 2, r->head_stride * 2}; }
@@ -244,10 +264,15 @@ int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype,
     p.group = (int32_t)(q->num_heads / shape->num_heads);
     p.scale_log2 = (float)(scale * 1.4426950408889634);
     const PagedPlan plan = plan_paged(shape, q->num_heads, batch);
-    p.splits = (int32_t)plan.splits;
+    p.few_rows = plan.few_rows;
+    p.few = plan.few_rule;
+    p.tiles = plan.tile_rule;
+    p.few_tile = (int32_t)plan.few_tile;
+    p.block_rows = kBlockRows;
+    p.parts = (int32_t)plan.parts;
     p.part_out = static_cast<float*>(workspace);
-    p.part_stat = reinterpret_cast<float2*>(p.part_out + batch->num_rows * q->num_heads * plan.splits * head_dim);
-    return attend(p, true, e4m3, plan.few, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
+    p.part_stat = reinterpret_cast<float2*>(p.part_out + batch->num_rows * q->num_heads * plan.parts * head_dim);
+    return attend(p, &plan, e4m3, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
 }
 
 int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig_rows* v, const kvmig_rows* out, int dtype,
@@ -271,8 +296,9 @@ int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig
     p.heads = (int32_t)q->num_heads;
     p.group = (int32_t)(q->num_heads / k->num_heads);
     p.scale_log2 = (float)(scale * 1.4426950408889634);
-    p.splits = 1;
-    return attend(p, false, false, false, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
+    p.parts = 1;
+    p.few = p.tiles = SplitRule{1, 1, 1};
+    return attend(p, nullptr, false, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
 }
 
 }  // extern "C"

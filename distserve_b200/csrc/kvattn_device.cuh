@@ -12,15 +12,26 @@ struct AttnRows {
     int64_t row_stride, head_stride;   // bytes
 };
 
+// How the keys of a sequence are cut into parts, each a block's work: in units of kSplitKeys keys, no part shorter than
+// `least` units nor than the whole call's work over `blocks`, and never more than `parts` of them.
+constexpr int kSplitKeys = 128;
+struct SplitRule {
+    int32_t parts, least, blocks;
+};
+
 struct AttnParams {
     AttnRows q, out, k, v;             // k, v: whole prompts only
     CacheView cache;
     BatchView batch;
     int32_t heads, group;              // query heads, query heads per KV head
     float scale_log2;                  // scale * log2(e): exponentials are taken to base 2
-    int32_t splits;                    // parts that a sequence's keys may be cut into, and their partial results:
-    float* part_out;                   // [row][head][split][head_dim], sums before the division
-    float2* part_stat;                 // [row][head][split]: running maximum (base 2) and sum
+    // Sequences of up to few_rows rows per KV head belong to the kernel for few rows, the others to the tile kernel.
+    int64_t few_rows;
+    SplitRule few, tiles;              // how each cuts a sequence's keys into parts
+    int32_t few_tile, block_rows;      // rows of a block of each
+    int32_t parts;                     // the parts' partial results, with room for this many:
+    float* part_out;                   // [row][head][part][head_dim], sums before the division
+    float2* part_stat;                 // [row][head][part]: running maximum (base 2) and sum
     int32_t box;                       // keys that the copy engine moves at once; 0: it cannot follow this layout
     int32_t q_box;                     // the same for Q: 1 if a tile of 128 rows is one box of tokens x query heads
     int32_t layers, layer;
@@ -31,18 +42,32 @@ struct AttnMaps {
     CUtensorMap k, v, q;
 };
 
-// Keys of one sequence that split s reads: whole units of kSplitKeys, dealt evenly; later splits may have none.
-constexpr int kSplitKeys = 128;
-struct KeyRange {
-    int begin, end;
-};
-__device__ __forceinline__ KeyRange split_range(int keys, int splits, int s) {
-    const int units = (keys + kSplitKeys - 1) / kSplitKeys, per = (units + splits - 1) / splits;
-    const int64_t begin = (int64_t)s * per * kSplitKeys;
-    KeyRange r;
-    r.begin = (int)min(begin, (int64_t)keys);
-    r.end = (int)min(begin + (int64_t)per * kSplitKeys, (int64_t)keys);
-    return r;
+// Row tiles of `tile` rows that a sequence has per KV head.
+__device__ __forceinline__ int64_t row_tiles(int64_t rows, int group, int tile) { return (rows * group + tile - 1) / tile; }
+
+// Units of a part, before `parts` is looked at: from the whole batch's work, which every warp that asks adds up.  TILES:
+// for the sequences of the tile kernel, else for those of the kernel for few rows.
+template <bool TILES>
+__device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, int tile) {
+    if (rule.parts == 1) return 0;
+    const int lane = threadIdx.x & 31, room = capacity(p.batch, p.cache);
+    unsigned long long sum = 0;
+    for (int i = lane; i < p.batch.num_seqs; i += 32) {
+        const Sequence s = sequence_at(p.batch, i);
+        if (s.rows == 0 || ((int64_t)s.rows * p.group > p.few_rows) != TILES) continue;
+        const unsigned units = (unsigned)(min(max(p.batch.seq_lens[i], 0), room) + kSplitKeys - 1) / kSplitKeys;
+        sum += units * (unsigned long long)row_tiles(s.rows, p.group, tile);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    sum = sum * (unsigned)(p.heads / p.group) / (unsigned)rule.blocks + 1;
+    return (int)(sum < (1u << 24) ? sum : (1u << 24));
+}
+
+// Keys of a part, for a sequence of `keys` of them.
+__device__ __forceinline__ int64_t part_keys(int keys, SplitRule rule, int units) {
+    const int all = (keys + kSplitKeys - 1) / kSplitKeys;
+    return (int64_t)max(max((all + rule.parts - 1) / rule.parts, rule.least), units) * kSplitKeys;
 }
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -90,14 +115,10 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two e4m3 codes (the low 16 bits) as two 16-bit values; exact.
-template <bool BF16>
+// Two e4m3 codes (the low 16 bits) as two 16-bit floats; exact.
 __device__ __forceinline__ uint32_t widen2(uint32_t codes) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3);
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
-    if (!BF16) return w;
-    const float2 f = Half<false>::to_float2(w);
-    return Half<true>::from_float2(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Pairs of 32-bit floats: one instruction for both.
@@ -114,6 +135,11 @@ __device__ __forceinline__ float2 unpair(uint64_t x) {
 __device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t x;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
+    return x;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t x;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
     return x;
 }
 __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {

@@ -1,12 +1,12 @@
 // Attention of few rows over the paged cache: a decoding step's single tokens and short drafts.
 //
-// A block takes the rows of one sequence that share a KV head, up to 16 of them (tokens x query heads of the group), and
-// one split of that sequence's keys.  Every K and V value is used for 16 rows at most, so the kernel is bound by reading
+// A block takes rows of one sequence that share a KV head, up to 16 or 32 of them (tokens x query heads of the group), and
+// one part of that sequence's keys.  Every K and V value is used for a few rows only, so the kernel is bound by reading
 // the cache; all else is arranged around keeping reads in flight:
 //   * each warp has its own ring of stages of 16 keys in shared memory, filled by cp.async and drained by that warp
 //     alone: no barrier of the block until the end, and about 96 KiB in flight per SM (two blocks);
 //   * warps take the groups of 16 keys in turn and keep their own running maximum, sum and output, joined at the end;
-//   * products run on m16n8k16 matrix instructions with the rows padded to 16.  Contraction order is free, so K
+//   * products run on m16n8k16 matrix instructions with the rows padded to 16 or 32.  Contraction order is free, so K
 //     fragments are read as 16 consecutive bytes per lane and Q's values are permuted to match, once;
 //   * e4m3 codes widen to 16 bits in registers; K's scales multiply the scores.  V's scale s_j goes into the exponent,
 //     P_j = 2^(score_j + log2 s_j - m), and the sum counts P_j / s_j: nothing can leave the 16-bit range that way.
@@ -16,62 +16,99 @@
 
 namespace kvmig {
 
-constexpr int kFewWarps = 4, kFewRows = 16, kFewKeys = 16;
+constexpr int kFewWarps = 4, kFewKeys = 16;
+constexpr int kFewMost = 64;          // rows of a sequence and KV head up to which this kernel is used
 
-template <int HD, bool E4M3> struct FewShape {
+template <int HD, bool E4M3, int MT> struct FewShape {
+    static constexpr int kRows = 16 * MT;
     static constexpr int kRowBytes = HD * (E4M3 ? 1 : 2);
     static constexpr int kTile = kFewKeys * kRowBytes;                          // K or V of one stage
     static constexpr int kStage = 2 * kTile + (E4M3 ? 2 * kFewKeys * 4 : 0);    // and the scales behind them
     static constexpr int kStages = 24576 / kStage < 8 ? 24576 / kStage : 8;
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kJoin = kFewRows * (HD + 2) * 4;                       // a warp's result, in its own ring
+    static constexpr int kJoin = kRows * (HD + 2) * 4;                       // a warp's result, in its own ring
     static constexpr int kShared = kFewWarps * (kRing > kJoin ? kRing : kJoin);
 };
 
-template <int HD, bool BF16, bool E4M3>
-__global__ void __launch_bounds__(kFewWarps * 32) attend_few(const __grid_constant__ AttnParams p) {
-    using S = FewShape<HD, E4M3>;
+template <int HD, bool BF16, bool E4M3, int MT>
+__global__ void __launch_bounds__(kFewWarps * 32, 2) attend_few(const __grid_constant__ AttnParams p) {
+    using S = FewShape<HD, E4M3, MT>;
     using H = Half<BF16>;
     constexpr int kSteps = HD / 16;                       // contraction steps of q . k
     constexpr int kChunks = S::kRowBytes / 16;            // 16-byte pieces of a cached row
     constexpr int kFlip = kChunks >= 8 ? 4 : 0;           // odd keys swap their 64-byte halves: no bank conflicts
     auto turn = [](int r) { return kChunks >= 8 ? r & 7 : (r >> 1) & 3; };   // V's pieces are turned by the key for ldmatrix
+    constexpr bool kBf16 = BF16 && !E4M3;                 // e4m3 codes widen to fp16 with one instruction, whatever Q's type
+    using In = Half<kBf16>;
     extern __shared__ __align__(128) unsigned char smem[];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, c = lane & 3;
-    const int kv_heads = p.heads / p.group;
-    const int kv_head = blockIdx.x % kv_heads, seq = blockIdx.x / kv_heads, split = blockIdx.y;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");             // the tile kernel's rows are others
+    const int kv_heads = p.heads / p.group, tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
+    const int tile = blockIdx.x % tiles, kv_head = blockIdx.x / tiles % kv_heads, seq = blockIdx.x / tiles / kv_heads, split = blockIdx.y;
     const Sequence s = sequence_at(p.batch, seq);
-    if (s.rows == 0) return;
+    const int64_t total = (int64_t)s.rows * p.group;
     const bool too_many = s.rows > p.batch.max_rows;
-    const int rows = too_many ? 0 : s.rows * p.group;     // rows of the tile: token * group + query head of the group
-    const int tokens = max(p.batch.seq_lens[seq], 0), first_pos = tokens - s.rows;   // position of the first row; may be negative
+    if (total <= (int64_t)tile * S::kRows || total > p.few_rows || (too_many && tile > 0)) return;
+    const int row0 = tile * S::kRows;                      // row r of the block: token (row0 + r) / group, query head % group
+    const int rows = too_many ? 0 : (int)min(total - row0, (int64_t)S::kRows);
+    const int tokens = max(p.batch.seq_lens[seq], 0), first_pos = tokens - s.rows;   // position of the first token; may be negative
     const int len = min(tokens, capacity(p.batch, p.cache));
-    KeyRange range = split_range(len, p.splits, split);
-    const bool whole = split_range(len, p.splits, 0).end == len;               // one split has everything
-    if (split > 0 && (whole || range.begin >= len)) return;
-    if (too_many) range.end = range.begin;
+    int64_t part = part_keys(len, p.few, 0);                                   // keys of a part
+    if (part * split < len) part = max(part, part_keys(len, p.few, part_units<false>(p, p.few, S::kRows)));
+    if (split > 0 && part * split >= len) return;
+    const bool whole = part >= len;                                            // one part has everything
+    struct { int begin, end; } range = {(int)(part * split), too_many ? 0 : (int)min(part * (split + 1), (int64_t)len)};
 
-    // Q: lane (quad, c) has rows quad and quad + 8.  16-bit pools: step t, values 32 (t/2) + 8 c + 4 (t%2) + 0..3;
+    // Q: lane (quad, c) has rows quad and quad + 8 of each 16.  16-bit pools: step t, values 32 (t/2) + 8 c + 4 (t%2) + 0..3;
     // quantised pools: 64 (t/4) + 16 c + 4 (t%4) + 0..3.
-    uint32_t q[kSteps][4];
+    uint32_t q[MT][kSteps][4];
+    int last[MT][2];                                       // the last key that each of the lane's rows sees
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int r = quad + half * 8;
-        const bool there = r < rows;
-        const char* at = p.q.data + (int64_t)(s.first + (there ? r / p.group : 0)) * p.q.row_stride +
-                         (int64_t)(kv_head * p.group + (there ? r % p.group : 0)) * p.q.head_stride;
+    for (int x = 0; x < MT; ++x)
 #pragma unroll
-        for (int t = 0; t < kSteps; ++t) {
-            const int d = E4M3 ? 64 * (t / 4) + 16 * c + 4 * (t % 4) : 32 * (t / 2) + 8 * c + 4 * (t % 2);
-            uint2 w = make_uint2(0, 0);
-            if (there) w = __ldg(reinterpret_cast<const uint2*>(at + d * 2));
-            q[t][half] = w.x;
-            q[t][half + 2] = w.y;
+        for (int half = 0; half < 2; ++half) {
+            const int r = x * 16 + quad + half * 8;
+            const bool there = r < rows;
+            const unsigned token = there ? (unsigned)(row0 + r) / (unsigned)p.group : 0, head = there ? (unsigned)(row0 + r) % (unsigned)p.group : 0;
+            last[x][half] = first_pos + (int)token;
+            const char* at = p.q.data + (int64_t)(s.first + (int)token) * p.q.row_stride + (int64_t)(kv_head * p.group + (int)head) * p.q.head_stride;
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t) {
+                const int d = E4M3 ? 64 * (t / 4) + 16 * c + 4 * (t % 4) : 32 * (t / 2) + 8 * c + 4 * (t % 2);
+                uint2 w = make_uint2(0, 0);
+                if (there) w = __ldg(reinterpret_cast<const uint2*>(at + d * 2));
+                q[x][t][half] = w.x;
+                q[x][t][half + 2] = w.y;
+            }
         }
-    }
-    // The last key that each of the lane's two rows sees.
-    const int last0 = first_pos + quad / p.group, last1 = first_pos + (quad + 8) / p.group;
+    // bf16 rows over a quantised pool go through fp16 times a power of two that brings the row's largest value to
+    // 2^14 .. 2^15: eight bits of fraction fit, and what is lost below 2^-24 is 2^-40 of that value.
+    float row_factor[MT][2];
+#pragma unroll
+    for (int x = 0; x < MT; ++x)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            row_factor[x][half] = p.scale_log2;
+            if (BF16 && E4M3) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t) top = __vmaxu2(top, __vmaxu2(q[x][t][half] & 0x7fff7fffu, q[x][t][half + 2] & 0x7fff7fffu));
+                top = max(top & 0xffffu, top >> 16);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = min(max((int)(top >> 7) - 127 - 14, -100), 112);     // of the largest value, minus 14
+                const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+                row_factor[x][half] *= __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const float2 f = Half<true>::to_float2(q[x][t][half + 2 * w]);
+                        q[x][t][half + 2 * w] = Half<false>::from_float2(f.x * up, f.y * up);
+                    }
+            }
+        }
 
     unsigned char* ring = smem + warp * (S::kShared / kFewWarps);
     const uint32_t ring_at = shared_address(ring);
@@ -120,144 +157,169 @@ __global__ void __launch_bounds__(kFewWarps * 32) attend_few(const __grid_consta
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; ++i) issue(i);
 
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // of rows quad and quad + 8
-    float o[HD / 8][4];
+    const int seen_by_all = min(first_pos + row0 / p.group + 1, range.end);    // keys before this one are seen by every row
+    float m[MT][2], l[MT][2], o[MT][HD / 8][4];             // of rows quad and quad + 8 of each 16
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
+    for (int x = 0; x < MT; ++x) {
+        m[x][0] = m[x][1] = -INFINITY;
+        l[x][0] = l[x][1] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-
+        for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[x][n][e] = 0.f;
+    }
     for (int i = 0; i < mine; ++i) {
         issue(i + S::kStages - 1);
         copy_wait<S::kStages - 1>();
         __syncwarp();
         const uint32_t k_at = ring_at + (i % S::kStages) * S::kStage, v_at = k_at + S::kTile;
-        // scores of 16 keys: tile n has keys 8 n + 2 c + {0, 1} of the lane's two rows
-        float sc[2][4] = {};
+        // scores of 16 keys: tile n has keys 8 n + 2 c + {0, 1} of the lane's rows
+        float sc[MT][2][4] = {};
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const int r = n * 8 + quad;
 #pragma unroll
             for (int j = 0; j < kChunks / 4; ++j) {
                 const uint4 w = load_shared16(k_at + r * S::kRowBytes + (((j * 4 + c) ^ ((r & 1) * kFlip)) * 16));
+                const uint32_t in[4] = {w.x, w.y, w.z, w.w};
                 if (E4M3) {
-                    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) mma_16x8x16<BF16>(sc[n], q[j * 4 + t], widen2<BF16>(in[t]), widen2<BF16>(in[t] >> 16));
+                    for (int t = 0; t < 4; ++t) {
+                        const uint32_t b0 = widen2(in[t]), b1 = widen2(in[t] >> 16);
+#pragma unroll
+                        for (int x = 0; x < MT; ++x) mma_16x8x16<kBf16>(sc[x][n], q[x][j * 4 + t], b0, b1);
+                    }
                 } else {
-                    mma_16x8x16<BF16>(sc[n], q[j * 2], w.x, w.y);
-                    mma_16x8x16<BF16>(sc[n], q[j * 2 + 1], w.z, w.w);
+#pragma unroll
+                    for (int x = 0; x < MT; ++x) {
+                        mma_16x8x16<kBf16>(sc[x][n], q[x][j * 2], in[0], in[1]);
+                        mma_16x8x16<kBf16>(sc[x][n], q[x][j * 2 + 1], in[2], in[3]);
+                    }
                 }
             }
         }
         const int key = first_key(i) + 2 * c;
-        float inverse[2][2];                                  // 1 / V's scale
+        float k_scale[2][2], lift[2][2], inverse[2][2];        // K's scale, log2 and inverse of V's scale
+        if (E4M3) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            float ks[2] = {p.scale_log2, p.scale_log2}, lift[2] = {0.f, 0.f};
-            if (E4M3) {
-                const float* scales = reinterpret_cast<const float*>(ring + (i % S::kStages) * S::kStage + 2 * S::kTile) + n * 8 + 2 * c;
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    ks[e] *= scales[e];
-                    lift[e] = __log2f(scales[16 + e]);
-                    inverse[n][e] = __fdividef(1.f, scales[16 + e]);
+                    const float* scales = reinterpret_cast<const float*>(ring + (i % S::kStages) * S::kStage + 2 * S::kTile) + n * 8 + 2 * c + e;
+                    k_scale[n][e] = scales[0];
+                    lift[n][e] = __log2f(scales[16]);
+                    inverse[n][e] = __fdividef(1.f, scales[16]);
                 }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int at = key + n * 8 + (e & 1), last = e < 2 ? last0 : last1;
-                const float x = sc[n][e] * ks[e & 1] + lift[e & 1];
-                sc[n][e] = at <= last && at < range.end ? x : -INFINITY;
-            }
         }
-        float top0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-        float top1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+        const bool all = first_key(i) + kFewKeys <= seen_by_all;               // every row sees all of these keys
+        uint32_t a[MT][4];
 #pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, d));
-            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, d));
-        }
-        top0 = fmaxf(m0, top0);
-        top1 = fmaxf(m1, top1);
-        if (__any_sync(0xffffffffu, top0 > m0 || top1 > m1)) {
-            const float keep0 = m0 == top0 ? 1.f : exp2_fast(m0 - top0), keep1 = m1 == top1 ? 1.f : exp2_fast(m1 - top1);
-            m0 = top0;
-            m1 = top1;
-            l0 *= keep0;
-            l1 *= keep1;
+        for (int x = 0; x < MT; ++x) {
+            float top[2] = {m[x][0], m[x][1]};
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n) {
-                o[n][0] *= keep0;
-                o[n][1] *= keep0;
-                o[n][2] *= keep1;
-                o[n][3] *= keep1;
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float y = sc[x][n][e] * (E4M3 ? row_factor[x][e / 2] * k_scale[n][e & 1] : row_factor[x][e / 2]);
+                    if (E4M3) y += lift[n][e & 1];
+                    const int at = key + n * 8 + (e & 1);
+                    if (!all) y = at <= last[x][e / 2] && at < range.end ? y : -INFINITY;
+                    sc[x][n][e] = y;
+                    top[e / 2] = fmaxf(top[e / 2], y);
+                }
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+            if (__any_sync(0xffffffffu, top[0] > m[x][0] || top[1] > m[x][1])) {
+                float keep[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    keep[h] = m[x][h] == top[h] ? 1.f : exp2_fast(m[x][h] - top[h]);
+                    m[x][h] = top[h];
+                    l[x][h] *= keep[h];
+                }
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[x][n][e] *= keep[e / 2];
             }
+            const float base[2] = {m[x][0] == -INFINITY ? 0.f : m[x][0], m[x][1] == -INFINITY ? 0.f : m[x][1]};   // a row without a key yet
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = exp2_fast(sc[x][n][e] - base[e / 2]);
+                    sc[x][n][e] = y;
+                    // a key that is not there may have any scale: it adds nothing
+                    l[x][e / 2] += E4M3 ? (y == 0.f ? 0.f : y * inverse[n][e & 1]) : y;
+                }
+            a[x][0] = In::from_float2(sc[x][0][0], sc[x][0][1]);
+            a[x][1] = In::from_float2(sc[x][0][2], sc[x][0][3]);
+            a[x][2] = In::from_float2(sc[x][1][0], sc[x][1][1]);
+            a[x][3] = In::from_float2(sc[x][1][2], sc[x][1][3]);
         }
-        const float base0 = m0 == -INFINITY ? 0.f : m0, base1 = m1 == -INFINITY ? 0.f : m1;   // a row that has seen no key yet
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sc[n][e] = exp2_fast(sc[n][e] - (e < 2 ? base0 : base1));
-                // a key that is not there may have any scale: it adds nothing
-                const float add = E4M3 ? (sc[n][e] == 0.f ? 0.f : sc[n][e] * inverse[n][e & 1]) : sc[n][e];
-                if (e < 2) l0 += add;
-                else l1 += add;
-            }
-        const uint32_t a[4] = {H::from_float2(sc[0][0], sc[0][1]), H::from_float2(sc[0][2], sc[0][3]),
-                               H::from_float2(sc[1][0], sc[1][1]), H::from_float2(sc[1][2], sc[1][3])};
         // o += P V: a lane gives ldmatrix the row of key (lane & 15), and the left or right of two neighbouring pieces
 #pragma unroll
         for (int j = 0; j < kChunks; j += 2) {
             const int r = lane & 15, piece = j + (lane >> 4);
             const uint4 w = load_matrices_transposed(v_at + r * S::kRowBytes + ((piece ^ turn(r)) * 16));
+            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
             if (E4M3) {
                 // a register has, for two keys, two neighbouring values each: even ones and odd ones make two tiles
-                const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    mma_16x8x16<BF16>(o[(j + x) * 2], a, widen2<BF16>(__byte_perm(in[2 * x], 0, 0x4420)), widen2<BF16>(__byte_perm(in[2 * x + 1], 0, 0x4420)));
-                    mma_16x8x16<BF16>(o[(j + x) * 2 + 1], a, widen2<BF16>(__byte_perm(in[2 * x], 0, 0x4431)), widen2<BF16>(__byte_perm(in[2 * x + 1], 0, 0x4431)));
+                for (int y = 0; y < 4; ++y) {
+                    const uint32_t pick = y & 1 ? 0x4431 : 0x4420;
+                    const uint32_t b0 = widen2(__byte_perm(in[y & 2], 0, pick)), b1 = widen2(__byte_perm(in[(y & 2) + 1], 0, pick));
+#pragma unroll
+                    for (int x = 0; x < MT; ++x) mma_16x8x16<kBf16>(o[x][j * 2 + y], a[x], b0, b1);
                 }
             } else {
-                mma_16x8x16<BF16>(o[j], a, w.x, w.y);
-                mma_16x8x16<BF16>(o[j + 1], a, w.z, w.w);
+#pragma unroll
+                for (int x = 0; x < MT; ++x) {
+                    mma_16x8x16<kBf16>(o[x][j], a[x], in[0], in[1]);
+                    mma_16x8x16<kBf16>(o[x][j + 1], a[x], in[2], in[3]);
+                }
             }
         }
         __syncwarp();                                          // the stage may be filled again
     }
     copy_wait<0>();
+    bad = __any_sync(0xffffffffu, bad);
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-    }
-    if (__any_sync(0xffffffffu, bad)) l0 = l1 = not_a_number();
+    for (int x = 0; x < MT; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], d);
+            if (bad) l[x][h] = not_a_number();
+        }
 
     // Join the warps: each leaves its maximum, sum and output in what was its ring.
     __syncwarp();
     float* join = reinterpret_cast<float*>(ring);
-    if (c == 0) {
-        join[quad * 2] = m0;
-        join[quad * 2 + 1] = l0;
-        join[(quad + 8) * 2] = m1;
-        join[(quad + 8) * 2 + 1] = l1;
-    }
-    float* out = join + kFewRows * 2;
+    float* out = join + S::kRows * 2;
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n) {
-        // columns of the lane's values: 8 n + 2 c + {0, 1}, or of the even/odd tiles 16 (n/2) + 4 c + n%2 + {0, 2}
-        const int d = E4M3 ? 16 * (n / 2) + 4 * c + n % 2 : 8 * n + 2 * c, step = E4M3 ? 2 : 1;
-        out[quad * HD + d] = o[n][0];
-        out[quad * HD + d + step] = o[n][1];
-        out[(quad + 8) * HD + d] = o[n][2];
-        out[(quad + 8) * HD + d + step] = o[n][3];
-    }
+    for (int x = 0; x < MT; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = x * 16 + quad + h * 8;
+            if (c == 0) {
+                join[r * 2] = m[x][h];
+                join[r * 2 + 1] = l[x][h];
+            }
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) {
+                // columns of the lane's values: 8 n + 2 c + {0, 1}, or of the even/odd tiles 16 (n/2) + 4 c + n%2 + {0, 2}
+                const int d = E4M3 ? 16 * (n / 2) + 4 * c + n % 2 : 8 * n + 2 * c, step = E4M3 ? 2 : 1;
+                out[r * HD + d] = o[x][n][2 * h];
+                out[r * HD + d + step] = o[x][n][2 * h + 1];
+            }
+        }
     __syncthreads();
-    const int64_t total = (int64_t)s.rows * p.group;          // all of a sequence's rows become NaN if there are too many
+    const int64_t written = too_many ? total : rows;          // all of a sequence's rows become NaN if there are too many
     constexpr int kPairs = HD / 2;
-    for (int64_t x = threadIdx.x; x < total * kPairs; x += kFewWarps * 32) {
+    for (int64_t x = threadIdx.x; x < written * kPairs; x += kFewWarps * 32) {
         const int64_t r = x / kPairs;
         const int d = (int)(x % kPairs) * 2, in = too_many ? 0 : (int)r;
         float m = -INFINITY;
@@ -269,25 +331,25 @@ __global__ void __launch_bounds__(kFewWarps * 32) attend_few(const __grid_consta
         for (int w = 0; w < kFewWarps; ++w) {
             const float* from = reinterpret_cast<const float*>(smem + w * (S::kShared / kFewWarps));
             const float f = exp2_fast(from[in * 2] - base);
-            const float2 v = *reinterpret_cast<const float2*>(from + kFewRows * 2 + in * HD + d);
+            const float2 v = *reinterpret_cast<const float2*>(from + S::kRows * 2 + in * HD + d);
             l += f * from[in * 2 + 1];
             a += f * v.x;
             b += f * v.y;
         }
-        const int64_t row = s.first + r / p.group, head = kv_head * p.group + r % p.group;
+        const int64_t row = s.first + (row0 + r) / p.group, head = kv_head * p.group + (row0 + r) % p.group;
         if (too_many || whole) {
             const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);           // no key: zeros; NaN stays
             if (split == 0)
                 *reinterpret_cast<uint32_t*>(p.out.data + row * p.out.row_stride + head * p.out.head_stride + d * 2) = H::from_float2(a * inv, b * inv);
         } else {
-            const int64_t part = (row * p.heads + head) * p.splits + split;
-            *reinterpret_cast<float2*>(p.part_out + part * HD + d) = make_float2(a, b);
-            if (d == 0) p.part_stat[part] = make_float2(m, l);
+            const int64_t place = (row * p.heads + head) * p.parts + split;
+            *reinterpret_cast<float2*>(p.part_out + place * HD + d) = make_float2(a, b);
+            if (d == 0) p.part_stat[place] = make_float2(m, l);
         }
     }
 }
 
-// Joins the splits' partial results, in their order: a warp per row and query head.
+// Joins the parts' partial results, in their order: a warp per row and query head.
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(128) attend_join(const __grid_constant__ AttnParams p) {
     constexpr int N = HD / 32;                                // values of a lane
@@ -299,12 +361,15 @@ __global__ void __launch_bounds__(128) attend_join(const __grid_constant__ AttnP
     const Sequence s = sequence_at(p.batch, seq);
     if (row < s.first || row - s.first >= s.rows || s.rows > p.batch.max_rows) return;
     const int len = min(max(p.batch.seq_lens[seq], 0), capacity(p.batch, p.cache));
-    if (split_range(len, p.splits, 0).end == len) return;     // written by its only split
-    const int64_t part = warp * p.splits;
+    const bool few = (int64_t)s.rows * p.group <= p.few_rows;
+    const int64_t per = few ? part_keys(len, p.few, part_units<false>(p, p.few, p.few_tile)) : part_keys(len, p.tiles, part_units<true>(p, p.tiles, p.block_rows));
+    if (per >= len) return;                                   // written by its only part
+    const int parts = (int)((len + per - 1) / per);
+    const int64_t part = warp * p.parts;
     float m = -INFINITY, l = 0.f, o[N] = {};
-    for (int i = 0; i < p.splits && split_range(len, p.splits, i).begin < len; ++i) m = fmaxf(m, p.part_stat[part + i].x);
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_stat[part + i].x);
     const float base = m == -INFINITY ? 0.f : m;
-    for (int i = 0; i < p.splits && split_range(len, p.splits, i).begin < len; ++i) {
+    for (int i = 0; i < parts; ++i) {
         const float2 stat = p.part_stat[part + i];
         const float f = exp2_fast(stat.x - base);
         l += f * stat.y;

@@ -42,14 +42,21 @@ template <bool BF16>
 __device__ __forceinline__ void widen16(const uint4& codes, float scale, uint4& lo, uint4& hi) {
     const uint32_t in[4] = {codes.x, codes.y, codes.z, codes.w};
     uint32_t out[8];
-    if (!BF16 && scale >= 5.9604644775390625e-08f && scale <= 128.f) {
+    if (!BF16 && scale >= 0x1p-24f && scale <= 128.f) {
         // the scale is a 16-bit value itself and no product leaves the range
         const __half2 s = __float2half2_rn(scale);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            uint32_t w = widen2<false>(in[j / 2] >> (j % 2 * 16));
+            uint32_t w = widen2(in[j / 2] >> (j % 2 * 16));
             const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&w), s);
             out[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    } else if (BF16 && scale <= 0x1p100f) {
+        const uint64_t s = pair(scale, scale);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 f = decode2(in[j / 2] >> (j % 2 * 16)), y = unpair(mul_pair(pair(f.x, f.y), s));
+            out[j] = Half<true>::from_float2(y.x, y.y);
         }
     } else {
         using H = Half<BF16>;
@@ -75,6 +82,10 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int j) {
 
 __device__ unsigned int g_attention_timeouts;      // blocks that gave up waiting
 
+// The grid may start while the grid before it, which it does not depend on, still runs, but must not end before it:
+// what follows in the stream waits for this one only.
+__device__ __forceinline__ void finish_after_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <int HD, bool BF16, bool PAGED, bool E4M3>
 __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_tiles(const __grid_constant__ AttnParams p, const __grid_constant__ AttnMaps maps) {
     using T = TileShape<HD, E4M3>;
@@ -98,7 +109,10 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
     const int tile = tiles - 1 - blockIdx.x / (kv_heads * p.batch.num_seqs), split = blockIdx.y;
     const Sequence s = sequence_at(p.batch, seq);
     const int64_t total = (int64_t)s.rows * p.group, row0 = (int64_t)tile * kBlockRows;
-    if (row0 >= total) return;
+    if (row0 >= total || total <= p.few_rows) {        // nothing here, or the other kernel's
+        finish_after_predecessor();
+        return;
+    }
     if (s.rows > p.batch.max_rows) {                   // more rows than the grid has tiles for
         if (tile == 0 && split == 0)
             for (int64_t x = threadIdx.x; x < total * (HD / 8); x += kTileThreads) {
@@ -107,13 +121,20 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
                                           (kv_head * p.group + r % p.group) * p.out.head_stride + x % (HD / 8) * 16) =
                     make_uint4(H::kNan2, H::kNan2, H::kNan2, H::kNan2);
             }
+        finish_after_predecessor();
         return;
     }
     const int tokens = PAGED ? max(p.batch.seq_lens[seq], 0) : s.rows, first_pos = tokens - s.rows;
     const int len = PAGED ? min(tokens, capacity(p.batch, p.cache)) : tokens;
-    const KeyRange range = split_range(len, p.splits, split);
-    const bool whole = split_range(len, p.splits, 0).end == len;
-    if (split > 0 && (whole || range.begin >= len)) return;
+    int64_t part = len;                                // keys of a part
+    if (PAGED) part = part_keys(len, p.tiles, 0);
+    if (PAGED && part * split < len) part = max(part, part_keys(len, p.tiles, part_units<true>(p, p.tiles, kBlockRows)));
+    if (split > 0 && part * split >= len) {
+        finish_after_predecessor();
+        return;
+    }
+    const bool whole = part >= len;
+    struct { int begin, end; } range = {(int)(part * split), (int)min(part * (split + 1), (int64_t)len)};
     // Row r of the block is token token0 + (skip + r) / group, query head (skip + r) % group of the group.
     const int token0 = (int)(row0 / p.group), here = (int)min((int64_t)kBlockRows, total - row0);
     const unsigned group = p.group, skip = (unsigned)(row0 - (int64_t)token0 * group);
@@ -254,9 +275,9 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
         if (!ok || flags[0] || flags[1]) l = not_a_number();
         const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
         const int64_t out_row = s.first + token, head = kv_head * group + (skip + threadIdx.x) % group;
-        const int64_t part = (out_row * p.heads + head) * p.splits + split;
+        const int64_t place = (out_row * p.heads + head) * p.parts + split;
         char* to = p.out.data + out_row * p.out.row_stride + head * p.out.head_stride;
-        if (there && !whole) p.part_stat[part] = make_float2(m, l);
+        if (there && !whole) p.part_stat[place] = make_float2(m, l);
 #pragma unroll
         for (int j = 0; j < HD; j += 32) {
             uint32_t o[32];
@@ -279,7 +300,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
             } else {
 #pragma unroll
                 for (int e = 0; e < 32; e += 4)
-                    *reinterpret_cast<uint4*>(p.part_out + part * HD + j + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    *reinterpret_cast<uint4*>(p.part_out + place * HD + j + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
         }
         tmem_fence_before();
@@ -566,6 +587,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
         tmem_fence_after();
         tmem_free(tmem, 512);
     }
+    finish_after_predecessor();
 }
 
 }  // namespace kvmig

@@ -133,15 +133,18 @@ class Expected:
     tol: torch.Tensor       # how far each value may be off
 
 
-def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, dtype: str) -> Expected:
+def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, dtype: str, quantised: bool = False) -> Expected:
     """q [Q, heads, D] at the last Q positions of k, v [S, kv_heads, D].
 
     The bound, per output, with h = eps / 2 of the 16-bit type and A = sum_j p_j |v_j|:
       h A                probabilities rounded to 16 bits before the second product
       h |o|              the same roundings where they enter the sum of the probabilities
       h |o|              the result's own rounding (plus half the type's smallest step)
-      2**-23 |v| summed  fp16 only: probabilities below 2**-14 are rounded absolutely, by 2**-25 at most, and the sum that
-                         divides them is at least 1/2
+      2**-23 |v| summed  where probabilities are rounded to fp16 (fp16 rows, and few rows over a quantised pool, whose e4m3
+                         codes widen to fp16): below 2**-14 they are rounded absolutely, by 2**-25 at most, and the sum
+                         that divides them is at least 1/2; over a quantised pool P_j carries V's scale s_j, so that
+                         the 2**-25 count 2**-25 |v_j| s_max / s_j, and s_max / s_j is at most 2 for rows drawn from one
+                         normal distribution (their largest magnitudes are within a factor of 2, or next to it)
       A 2**-24 (2 E + n + 64)   32-bit sums over n keys, exponentials, and scores that are off by at most
                          E = (D + 2) scale sum |q k| units of 2**-24, numerator and denominator alike
     """
@@ -161,16 +164,15 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, dtyp
     h = torch.finfo(DTYPES[dtype]).eps / 2
     big = torch.einsum("hqs,shd->qhd", p, vv.abs())
     visible = (~hidden).double()[None].expand(heads, -1, -1)
-    absolute = 2.0 ** -23 * torch.einsum("hqs,shd->qhd", visible, vv.abs()) if dtype == "fp16" else 0.0
+    absolute = 2.0 ** -23 * torch.einsum("hqs,shd->qhd", visible, vv.abs()) if dtype == "fp16" or quantised else 0.0
     size = abs(scale) * torch.einsum("qhd,shd->hqs", qd.abs(), kk.abs())
     size = (size * visible).amax(-1).transpose(0, 1)[..., None] if k.shape[0] else 0.0
     tol = h * (big + 2 * out.abs()) + absolute + big * 2.0 ** -24 * (2 * (dim + 2) * size + k.shape[0] + 64)
-    return Expected(out, tol * 1.01 + torch.finfo(DTYPES[dtype]).smallest_subnormal if hasattr(torch.finfo(DTYPES[dtype]), "smallest_subnormal")
-                    else tol * 1.01 + torch.finfo(DTYPES[dtype]).tiny)
+    return Expected(out, tol * 1.01 + torch.finfo(DTYPES[dtype]).tiny * torch.finfo(DTYPES[dtype]).eps)
 
 
 def attend_paged(p: Paged, q: torch.Tensor, scale: float, dtype: str) -> List[Expected]:
-    return [attend(q[a:b], rows_of(p, p.k_cache, i), rows_of(p, p.v_cache, i), scale, dtype)
+    return [attend(q[a:b], rows_of(p, p.k_cache, i), rows_of(p, p.v_cache, i), scale, dtype, p.k_cache.dtype == torch.uint8)
             for i, (a, b) in enumerate(zip(p.starts.tolist(), p.starts.tolist()[1:]))]
 
 
