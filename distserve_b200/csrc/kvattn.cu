@@ -35,19 +35,22 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
     plan.few_rows = !plan.tiles ? INT64_MAX : plan.few ? kFewMost : 0;
     plan.few_tile = most <= 16 ? 16 : 32;
     const int64_t kv_heads = shape->num_heads, head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
-    // A part is at least the call's work over the blocks that the device holds at once (see part_units), so a sequence
-    // has no more parts than `fill`; the grid has a block for each, of which most return at once when there are many
-    // sequences, hence the bound by their number; and partial results stay below 256 MB.
+    // A part is at least the call's work over the blocks that the device holds at once (part_units); the device adds the
+    // work up, and the grid has room for the parts of the longest sequence if the others are a quarter as long.  Most of
+    // that room's blocks return at once when there are many sequences, hence the bound by their number; and partial
+    // results stay below 256 MB.
     const int64_t room = std::max<int64_t>((256 << 20) / std::max<int64_t>(b->num_rows * heads * (head_dim * 4 + 8), 1), 1);
-    auto rule = [&](int64_t blocks, int64_t least, int64_t most_blocks, int64_t tiles) {
-        const int64_t fill = blocks / kv_heads + 1, grid = most_blocks / std::max<int64_t>(b->num_seqs * kv_heads * tiles, 1);
-        const int64_t parts = std::min(std::min(units / least, fill), std::min(grid, room));
+    auto rule = [&](int64_t blocks, int64_t least, int64_t most_blocks, int64_t row_tiles) {
+        const int64_t n = std::max<int64_t>(b->num_seqs, 1), work = row_tiles * kv_heads * units * (n + 3) / (4 * n);
+        const int64_t part = std::max(least, work / blocks + 1), grid = most_blocks / std::max<int64_t>(row_tiles * kv_heads, 1);
+        // joining takes a launch of its own, which two parts of a short sequence are not worth
+        const int64_t parts = units <= 2 * least ? 1 : std::min(std::min((units + part - 1) / part, grid), room);
         return SplitRule{(int32_t)std::max<int64_t>(parts, 1), (int32_t)least, (int32_t)blocks};
     };
     plan.few_rule = plan.tile_rule = SplitRule{1, 1, 1};
-    if (plan.few) plan.few_rule = rule(2 * kSms, 2, 4096, (std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile);
+    if (plan.few) plan.few_rule = rule(2 * kSms, 4, 4096, b->num_seqs * ((std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile));
     // A block of the tile kernel has an SM to itself; twice as many parts even out sequences of different lengths.
-    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, 16384, 1);
+    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, 4096, b->num_rows * group / kBlockRows + b->num_seqs);
     plan.parts = std::max(plan.few_rule.parts, plan.tile_rule.parts);
     if (plan.parts > 1) plan.workspace = b->num_rows * heads * plan.parts * (head_dim * 4 + (int64_t)sizeof(float2));
     return plan;
@@ -56,6 +59,22 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
 BatchView batch_view(const kvmig_batch* batch) {
     return BatchView{batch->starts, batch->seq_lens, batch->block_tables, batch->table_stride, (int32_t)batch->num_seqs,
                      (int32_t)batch->num_rows, (int32_t)batch->max_rows, (int32_t)batch->max_blocks};
+}
+
+// Launches a grid that may begin, if `early`, once every block of the stream's previous grid has begun.
+template <typename... Args>
+cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, bool early, cudaStream_t stream, const Args&... args) {
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 template <int HD, bool BF16, bool E4M3, int MT>
@@ -144,17 +163,8 @@ int launch_tiles(const AttnParams& params, bool after_few, cudaStream_t stream, 
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     // After the kernel for few rows, which has other rows to do: begins when that one's blocks leave room.
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)grid, p.tiles.parts);
-    config.blockDim = dim3(TileShape<HD, E4M3>::kThreads);
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    config.attrs = &early;
-    config.numAttrs = after_few ? 1 : 0;
-    CU_TRY(cudaLaunchKernelEx(&config, attend_tiles<HD, BF16, PAGED, E4M3>, p, maps));
+    CU_TRY(launch_early(attend_tiles<HD, BF16, PAGED, E4M3>, dim3((unsigned)grid, p.tiles.parts), TileShape<HD, E4M3>::kThreads, smem, after_few,
+                        stream, p, maps));
     g_attention_launches++;
     return 0;
 }
@@ -167,10 +177,11 @@ int launch_paged(const AttnParams& p, const PagedPlan& plan, cudaStream_t stream
     }
     if (!rc && plan.tiles) rc = launch_tiles<HD, BF16, true, E4M3>(p, plan.few, stream, what);
     if (rc || p.parts == 1) return rc;
-    const int64_t grid = ((int64_t)p.batch.num_rows * p.heads + 3) / 4;
-    if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
-    attend_join<HD, BF16><<<(unsigned)grid, 128, 0, stream>>>(p);
-    CU_TRY(cudaGetLastError());
+    // A block for each result while they fit the device at once, else a warp for each.
+    const int64_t items = (int64_t)p.batch.num_rows * p.heads, most = 8 * kSms;
+    const bool wide = items <= most;
+    CU_TRY(launch_early(wide ? attend_join<HD, BF16, true> : attend_join<HD, BF16, false>,
+                        dim3((unsigned)std::min(wide ? items : (items + kJoinWarps - 1) / kJoinWarps, most)), kJoinThreads, 0, true, stream, p));
     g_attention_launches++;
     return 0;
 }

@@ -42,26 +42,31 @@ struct AttnMaps {
     CUtensorMap k, v, q;
 };
 
-// Row tiles of `tile` rows that a sequence has per KV head.
-__device__ __forceinline__ int64_t row_tiles(int64_t rows, int group, int tile) { return (rows * group + tile - 1) / tile; }
-
 // Units of a part, before `parts` is looked at: from the whole batch's work, which every warp that asks adds up.  TILES:
-// for the sequences of the tile kernel, else for those of the kernel for few rows.
+// for the sequences of the tile kernel, else for those of the kernel for few rows.  With t row tiles in all, cutting to
+// work / (blocks - t) units leaves no more than `blocks` parts, whatever the lengths.
 template <bool TILES>
 __device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, int tile) {
     if (rule.parts == 1) return 0;
-    const int lane = threadIdx.x & 31, room = capacity(p.batch, p.cache);
+    const int lane = threadIdx.x & 31, room = capacity(p.batch, p.cache), kv_heads = p.heads / p.group;
     unsigned long long sum = 0;
+    unsigned tiles = 0;
     for (int i = lane; i < p.batch.num_seqs; i += 32) {
         const Sequence s = sequence_at(p.batch, i);
+        const int tokens = p.batch.seq_lens[i];
         if (s.rows == 0 || ((int64_t)s.rows * p.group > p.few_rows) != TILES) continue;
-        const unsigned units = (unsigned)(min(max(p.batch.seq_lens[i], 0), room) + kSplitKeys - 1) / kSplitKeys;
-        sum += units * (unsigned long long)row_tiles(s.rows, p.group, tile);
+        const unsigned units = (unsigned)(min(max(tokens, 0), room) + kSplitKeys - 1) / kSplitKeys;
+        const unsigned n = (unsigned)min(((int64_t)s.rows * p.group + tile - 1) / tile, (int64_t)1 << 20);
+        sum += units * (unsigned long long)n;
+        tiles += n;
     }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    sum = sum * (unsigned)(p.heads / p.group) / (unsigned)rule.blocks + 1;
-    return (int)(sum < (1u << 24) ? sum : (1u << 24));
+    for (int d = 16; d; d >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+    }
+    const float blocks = fmaxf((float)rule.blocks - (float)tiles * kv_heads, 0.5f * rule.blocks);
+    return (int)fminf((float)sum * kv_heads / blocks, 1e6f) + 1;
 }
 
 // Keys of a part, for a sequence of `keys` of them.

@@ -349,42 +349,67 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attend_few(const __grid_con
     }
 }
 
-// Joins the parts' partial results, in their order: a warp per row and query head.
-template <int HD, bool BF16>
-__global__ void __launch_bounds__(128) attend_join(const __grid_constant__ AttnParams p) {
+// Joins the parts' partial results, in their order.  WIDE: a block per row and query head, whose warps share the parts;
+// else a warp for each.  No more blocks than the device holds at once, so that most warps find the batch in the
+// first-level cache.  The grid begins while its predecessor still runs and waits for it before it reads results.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+template <int HD, bool BF16, bool WIDE>
+__global__ void __launch_bounds__(kJoinThreads) attend_join(const __grid_constant__ AttnParams p) {
     constexpr int N = HD / 32;                                // values of a lane
-    const int lane = threadIdx.x & 31;
-    const int64_t warp = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), row64 = warp / p.heads;
-    if (row64 >= p.batch.num_rows) return;
-    const int row = (int)row64, head = (int)(warp % p.heads);
-    const int seq = find_sequence(p.batch.starts, p.batch.num_seqs, row);
-    const Sequence s = sequence_at(p.batch, seq);
-    if (row < s.first || row - s.first >= s.rows || s.rows > p.batch.max_rows) return;
-    const int len = min(max(p.batch.seq_lens[seq], 0), capacity(p.batch, p.cache));
-    const bool few = (int64_t)s.rows * p.group <= p.few_rows;
-    const int64_t per = few ? part_keys(len, p.few, part_units<false>(p, p.few, p.few_tile)) : part_keys(len, p.tiles, part_units<true>(p, p.tiles, p.block_rows));
-    if (per >= len) return;                                   // written by its only part
-    const int parts = (int)((len + per - 1) / per);
-    const int64_t part = warp * p.parts;
-    float m = -INFINITY, l = 0.f, o[N] = {};
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_stat[part + i].x);
-    const float base = m == -INFINITY ? 0.f : m;
-    for (int i = 0; i < parts; ++i) {
-        const float2 stat = p.part_stat[part + i];
-        const float f = exp2_fast(stat.x - base);
-        l += f * stat.y;
-        const float* from = p.part_out + (part + i) * HD + lane * N;
+    __shared__ float shared[WIDE ? kJoinWarps * (HD + 2) : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = WIDE ? warp : 0, step = WIDE ? kJoinWarps : 1;
+    const int few_units = part_units<false>(p, p.few, p.few_tile), tile_units = part_units<true>(p, p.tiles, p.block_rows);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t items = (int64_t)p.batch.num_rows * p.heads, stride = (int64_t)gridDim.x * (WIDE ? 1 : kJoinWarps);
+    for (int64_t item = (int64_t)blockIdx.x * (WIDE ? 1 : kJoinWarps) + (WIDE ? 0 : warp); item < items; item += stride) {
+        const int row = (int)(item / p.heads), head = (int)(item % p.heads);
+        const int seq = find_sequence(p.batch.starts, p.batch.num_seqs, row);
+        const Sequence s = sequence_at(p.batch, seq);
+        if (row < s.first || row - s.first >= s.rows || s.rows > p.batch.max_rows) continue;
+        const int len = min(max(p.batch.seq_lens[seq], 0), capacity(p.batch, p.cache));
+        const bool few = (int64_t)s.rows * p.group <= p.few_rows;
+        const int64_t per = part_keys(len, few ? p.few : p.tiles, few ? few_units : tile_units);
+        if (per >= len) continue;                             // written by its only part
+        const int parts = (int)((len + per - 1) / per);
+        const int64_t place = item * p.parts;
+        float m = -INFINITY, l = 0.f, o[N] = {};
+        for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_stat[place + i].x);
 #pragma unroll
-        for (int n = 0; n < N; n += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(from + n);
-            o[n] += f * v.x;
-            o[n + 1] += f * v.y;
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+        for (int i = first; i < parts; i += step) {
+            const float2 stat = p.part_stat[place + i];
+            const float f = exp2_fast(stat.x - base);
+            l += f * stat.y;
+            const float* from = p.part_out + (place + i) * HD + lane * N;
+#pragma unroll
+            for (int n = 0; n < N; n += 2) {
+                const float2 v = *reinterpret_cast<const float2*>(from + n);
+                o[n] += f * v.x;
+                o[n + 1] += f * v.y;
+            }
         }
-    }
-    const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
-    uint32_t* to = reinterpret_cast<uint32_t*>(p.out.data + (int64_t)row * p.out.row_stride + (int64_t)head * p.out.head_stride) + lane * (N / 2);
+        if (WIDE) {
+            __syncthreads();                                  // the previous item has been read
+            float* mine = shared + warp * (HD + 2);
+            if (lane == 0) mine[HD] = l;
 #pragma unroll
-    for (int n = 0; n < N; n += 2) to[n / 2] = Half<BF16>::from_float2(o[n] * inv, o[n + 1] * inv);
+            for (int n = 0; n < N; ++n) mine[lane * N + n] = o[n];
+            __syncthreads();
+            if (warp > 0) continue;
+#pragma unroll
+            for (int w = 1; w < kJoinWarps; ++w) {
+                l += shared[w * (HD + 2) + HD];
+#pragma unroll
+                for (int n = 0; n < N; ++n) o[n] += shared[w * (HD + 2) + lane * N + n];
+            }
+        }
+        const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
+        uint32_t* to = reinterpret_cast<uint32_t*>(p.out.data + (int64_t)row * p.out.row_stride + (int64_t)head * p.out.head_stride) + lane * (N / 2);
+#pragma unroll
+        for (int n = 0; n < N; n += 2) to[n / 2] = Half<BF16>::from_float2(o[n] * inv, o[n + 1] * inv);
+    }
 }
 
 }  // namespace kvmig

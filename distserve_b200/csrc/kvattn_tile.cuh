@@ -102,6 +102,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
                    drained = pv_done + 16, raw_full = drained + 8, raw_empty = raw_full + T::kRawSlots * 8;
     volatile int* flags = reinterpret_cast<volatile int*>(smem + T::kBars + T::kBarriers * 8);    // failed, bad, tensor memory
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");             // the join waits for the end of this grid
     // Which rows and keys.  Later row tiles, which have more keys, come first.
     const int kv_heads = p.heads / p.group;
     const int tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
         barrier_init(q_full, kLoadWarps);
         barrier_init(drained, 1);
         for (int i = 0; i < T::kRawSlots; ++i) {
-            barrier_init(raw_full + i * 8, 1);
+            barrier_init(raw_full + i * 8, kLoadWarps);
             barrier_init(raw_empty + i * 8, kLoadWarps);
         }
         for (int t = 0; t < 2; ++t) {
@@ -236,9 +237,17 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
                 if (lane == 0) barrier_arrive(bar);
             };
             uint32_t w[32];
-            // Every step begins with the maximum so far, as if this tile did not raise it beyond the allowance.
+            // Every step but the first begins with the maximum so far, as if this tile did not raise it beyond the allowance.
             uint64_t shift2 = pair(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
-            probabilities(a, w, shift2, true);
+            if (i > 0) {
+                probabilities(a, w, shift2, true);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    tops[j % 2] = max_nan(tops[j % 2], __uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1]));
+                    tops[j % 2 + 2] = max_nan(tops[j % 2 + 2], __uint_as_float(b[2 * j]), __uint_as_float(b[2 * j + 1]));
+                }
+            }
             const float top = max_nan(max_nan(tops[0], tops[1], tops[2]), tops[3], -INFINITY) * scale;
             const bool grown = i == 0 || !(top <= m + kLazy);
             if (__any_sync(0xffffffffu, grown)) {
@@ -342,7 +351,28 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
         // Whole tiles go through the copy engine where it can follow the layout; the last one of a sequence, whose
         // missing keys have to be zeros, and other layouts are copied 16 bytes at a time.
         auto by_engine = [&](int c) { return p.box > 0 && range.begin + (c / 2 + 1) * kTileKeys <= range.end; };
-        const int boxes = p.box > 0 ? kTileKeys / p.box : 1;
+        // The engine's copies of a paged tile are dealt over the loading warps, one to a lane: box `box_of` of the tile and
+        // its left or right 64 values (codes or scales for quantised pools).  Block ids are read a step ahead.
+        constexpr int kPerBox = E4M3 ? 2 : HD / 64;
+        const int deal = lane * kLoadWarps + w, box_of = deal / kPerBox, part_of = deal % kPerBox;
+        const bool dealt = PAGED && p.box > 0 && box_of < kTileKeys / max(p.box, 1);
+        int ahead = -1;
+        auto look_ahead = [&](int i) {
+            const int key = range.begin + i * kTileKeys + box_of * p.box;
+            ahead = -1;
+            if (dealt && range.begin + (i + 1) * kTileKeys <= range.end && key / p.cache.block_size < p.batch.max_blocks)
+                ahead = p.batch.block_tables[seq * p.batch.table_stride + key / p.cache.block_size];
+        };
+        int id = -1;                                                    // this lane's block in the current step
+        auto engine_block = [&](int c) {
+            if (c % 2 == 0) {
+                id = (unsigned)ahead < (unsigned)p.cache.num_blocks ? ahead : -1;
+                bad |= dealt && id < 0;
+                look_ahead(c / 2 + 1);
+            }
+            return dealt && id >= 0;
+        };
+        if (PAGED) look_ahead(0);
         // Byte offsets of four keys of a tile, r = lane + 32 x; -1 if there is no such key.
         int64_t at_k[4], at_v[4];
         auto look_up = [&](int i) {
@@ -379,25 +409,23 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
                     if (by_engine(c)) {
                         const void* map = c % 2 ? &maps.v : &maps.k;
                         const int key = range.begin + c / 2 * kTileKeys;
-                        if (w > 0) {
-                            if (lane == 0) barrier_arrive(full(slot));
-                        } else if (!PAGED) {
+                        if (!PAGED) {
                             if (lane == 0) {
-                                barrier_expect(full(slot), T::kSlot);
-                                for (int h = 0; h < HD / 64; ++h) box_copy(to + h * kTileKeys * 128, map, h * 64, kv_head, s.first + key, full(slot));
+                                if (w > 0) {
+                                    barrier_arrive(full(slot));
+                                } else {
+                                    barrier_expect(full(slot), T::kSlot);
+                                    for (int h = 0; h < HD / 64; ++h) box_copy(to + h * kTileKeys * 128, map, h * 64, kv_head, s.first + key, full(slot));
+                                }
                             }
                         } else {
-                            const int b = lane / (HD / 64), h = lane % (HD / 64), first = key + b * p.box;
-                            int id = -1;
-                            if (b < boxes) id = block_of(p.batch, p.cache, seq, first);
-                            const bool there = b < boxes && id >= 0;
-                            bad |= b < boxes && id < 0;
+                            const bool there = engine_block(c);
                             const int copies = __popc(__ballot_sync(0xffffffffu, there));
                             if (lane == 0) barrier_expect(full(slot), copies * p.box * 128);
                             __syncwarp();
                             if (there)
-                                box_copy(to + h * kTileKeys * 128 + b * p.box * 128, map, h * 64,
-                                         ((id * p.layers + p.layer) * kv_heads + kv_head) * p.cache.block_size + first % p.cache.block_size, full(slot));
+                                box_copy(to + part_of * kTileKeys * 128 + box_of * p.box * 128, map, part_of * 64,
+                                         ((id * p.layers + p.layer) * kv_heads + kv_head) * p.cache.block_size + (key + box_of * p.box) % p.cache.block_size, full(slot));
                         }
                     } else {
                         look_up(c / 2);
@@ -428,23 +456,18 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
                     const uint32_t to = base + T::kRaw + slot * T::kRawSlot;
                     const char* data = c % 2 ? v_data : k_data;
                     if (by_engine(c)) {
-                        if (w > 0) return;
                         if (c >= T::kRawSlots && !(ok = warp_wait(raw_empty + slot * 8, (c / T::kRawSlots - 1) & 1))) return;
-                        const int b = lane >> 1, first = range.begin + c / 2 * kTileKeys + b * p.box;
-                        int id = -1;
-                        if (b < boxes) id = block_of(p.batch, p.cache, seq, first);
-                        const bool there = b < boxes && id >= 0;
-                        bad |= b < boxes && id < 0;
-                        const int copies = __popc(__ballot_sync(0xffffffffu, there)) / 2;
-                        if (lane == 0) barrier_expect(raw_full + slot * 8, copies * p.box * (HD + 4));
+                        const bool there = engine_block(c);
+                        const int offset = (range.begin + c / 2 * kTileKeys + box_of * p.box) % p.cache.block_size;
+                        const uint32_t bytes = part_of ? p.box * 4 : p.box * HD, sum = __reduce_add_sync(0xffffffffu, there ? bytes : 0);
+                        if (lane == 0) barrier_expect(raw_full + slot * 8, sum);
                         __syncwarp();
                         if (there) {
                             const char* tile_at = data + id * p.cache.block_stride + (int64_t)kv_head * p.cache.head_stride;
-                            const int offset = first % p.cache.block_size;
-                            if (lane & 1)
-                                bulk_copy(to + kTileKeys * HD + b * p.box * 4, tile_at + (int64_t)p.cache.block_size * HD + offset * 4, p.box * 4, raw_full + slot * 8);
+                            if (part_of)
+                                bulk_copy(to + kTileKeys * HD + box_of * p.box * 4, tile_at + (int64_t)p.cache.block_size * HD + offset * 4, bytes, raw_full + slot * 8);
                             else
-                                bulk_copy(to + b * p.box * HD, tile_at + (int64_t)offset * HD, p.box * HD, raw_full + slot * 8);
+                                bulk_copy(to + box_of * p.box * HD, tile_at + (int64_t)offset * HD, bytes, raw_full + slot * 8);
                         }
                         return;
                     }
