@@ -120,39 +120,6 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two e4m3 codes (the low 16 bits) as two 16-bit floats; exact.
-__device__ __forceinline__ uint32_t widen2(uint32_t codes) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Pairs of 32-bit floats: one instruction for both.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t x;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
-    return x;
-}
-__device__ __forceinline__ float2 unpair(uint64_t x) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(x));
-    return f;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t x;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
-    return x;
-}
-__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
-    uint64_t x;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
-    return x;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-    uint64_t x;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
-    return x;
-}
-
 // The larger of three, NaN if one of them is.
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
     float x;

@@ -37,44 +37,6 @@ template <int HD, bool E4M3> struct TileShape {
     static constexpr int kShared = kBars + kBarriers * 8 + 32 + 1024;       // and room to align the start to 1024
 };
 
-// 16 e4m3 codes times their row's scale as 16-bit values: exactly what kvmig_cache_read gives.
-template <bool BF16>
-__device__ __forceinline__ void widen16(const uint4& codes, float scale, uint4& lo, uint4& hi) {
-    const uint32_t in[4] = {codes.x, codes.y, codes.z, codes.w};
-    uint32_t out[8];
-    if (!BF16 && scale >= 0x1p-24f && scale <= 128.f) {
-        // the scale is a 16-bit value itself and no product leaves the range
-        const __half2 s = __float2half2_rn(scale);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            uint32_t w = widen2(in[j / 2] >> (j % 2 * 16));
-            const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&w), s);
-            out[j] = *reinterpret_cast<const uint32_t*>(&x);
-        }
-    } else if (BF16 && scale <= 0x1p100f) {
-        const uint64_t s = pair(scale, scale);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 f = decode2(in[j / 2] >> (j % 2 * 16)), y = unpair(mul_pair(pair(f.x, f.y), s));
-            out[j] = Half<true>::from_float2(y.x, y.y);
-        }
-    } else {
-        using H = Half<BF16>;
-        const float top = H::largest();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float2 f = decode2(in[j / 2] >> (j % 2 * 16));
-            f.x *= scale;
-            f.y *= scale;
-            f.x = f.x > top ? top : f.x < -top ? -top : f.x;
-            f.y = f.y > top ? top : f.y < -top ? -top : f.y;
-            out[j] = H::from_float2(f.x, f.y);
-        }
-    }
-    lo = make_uint4(out[0], out[1], out[2], out[3]);
-    hi = make_uint4(out[4], out[5], out[6], out[7]);
-}
-
 // Byte offset of 16-byte piece j of row r in a tile: columns of 64 values, 128-byte rows, swizzled.
 __device__ __forceinline__ uint32_t tile_offset(int r, int j) {
     return (uint32_t)((j >> 3) * (kTileKeys * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4));

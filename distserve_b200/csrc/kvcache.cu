@@ -1,12 +1,17 @@
 // Writing new tokens' K and V rows into one layer of the paged pools and reading sequences back, in the pools' own
 // 16-bit type or quantised to e4m3 with a power-of-two scale per row (layout and definition: include/kvmig.h).
 //
-// Both are copies: what bounds them is HBM for long calls and launch latency for a decoding step's.  A warp owns a
-// part of ONE token, so the sequence, the position and the block are found once per warp, and moves 16 bytes per lane
-// and access.
+// Both are copies: what bounds them is HBM for long calls and launch latency for a decoding step's.  A warp works on one
+// token, so that sequence, position and block are found once per warp, and takes the token's rows in batches whose loads
+// are all issued before the first is used; a token's batches are shared between as many warps as fill the device several
+// times over.  Measured: 9.6k tokens of 40 heads quantised in 59.5 us (5.0 TB/s), 34k tokens of 4 heads read back in
+// 25.3 us (4.2 TB/s).  Two accesses a batch and blocks of 128 threads were best (1: 61.6 / 25.4 us, 4: 62.6 / 31.2;
+// blocks of 256: 59.7 / 26.6); warps that take 4 or 16 neighbouring tokens, so that a tile is read in longer runs, lose
+// (71 / 29 us).
 #include "kvcache_device.cuh"
 #include "kvmig_common.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace kvmig {
@@ -61,7 +66,7 @@ int check_pools(const void* k_cache, const void* v_cache, const kvmig_pool_shape
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct RowsView {
     char* data;
@@ -73,133 +78,139 @@ struct MoveParams {
     CacheView cache;
     BatchView batch;
     int32_t heads, head_dim;
-    int32_t parts;                     // warps per token
+    int32_t parts, batches;            // warps per token, and the batches that they share
 };
 
-// Elements of 16 bytes (16-bit pools) or rows (quantised pools) that a warp moves per access, times this many accesses.
-constexpr int kUnroll = 4;
+constexpr int64_t kFillWarps = 148 * 192;
+constexpr int kUnroll = 2;             // accesses of a batch, per lane
 
 struct Place {
-    int token, part, offset;           // offset of the token in its block
-    int64_t block;                     // byte offset of the block in the pool; -1: no such block
-    bool named;                        // a sequence of the batch has this row and a position for it
+    int64_t block;                     // byte offset of the block in the pool; -1: there is none, -2: nothing to do here
+    int offset;                        // of the token in its block
 };
 
 template <bool WRITE>
-__device__ __forceinline__ Place find_place(const MoveParams& p) {
-    const int64_t warp = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    Place at;
-    at.named = false;
-    at.token = (int)min(warp / p.parts, (int64_t)INT32_MAX);
-    at.part = (int)(warp % p.parts);
-    if (at.token >= p.batch.num_rows) return at;
-    const int i = find_sequence(p.batch.starts, p.batch.num_seqs, at.token);
+__device__ __forceinline__ Place find_place(const MoveParams& p, int token) {
+    Place at{-2, 0};
+    const int i = find_sequence(p.batch.starts, p.batch.num_seqs, token);
     const Sequence s = sequence_at(p.batch, i);
-    int64_t pos = (int64_t)at.token - s.first;
+    int64_t pos = (int64_t)token - s.first;
     if (!s.valid || pos < 0 || pos >= s.rows) return at;
     if (WRITE) pos += (int64_t)p.batch.seq_lens[i] - s.rows;
     if (pos < 0) return at;
-    at.named = true;
     const int id = pos <= INT32_MAX ? block_of(p.batch, p.cache, i, (int)pos) : -1;
-    at.block = id < 0 ? -1 : id * p.cache.block_stride;
+    if (id < 0) at.block = WRITE ? -2 : -1;
+    else at.block = id * p.cache.block_stride;
     at.offset = (int)(pos % p.cache.block_size);
     return at;
 }
 
-// 16-bit pools.  The token's K and V are 2 * heads * head_dim / 8 pieces of 16 bytes; a warp takes 32 * kUnroll of them.
+// 16-bit pools.  A token's K and V are 2 * heads * head_dim / 8 pieces of 16 bytes; a batch is 32 * kUnroll pieces.
 template <bool WRITE>
 __global__ void __launch_bounds__(kThreads) kv_cache_move(const __grid_constant__ MoveParams p) {
-    const Place at = find_place<WRITE>(p);
-    if (!at.named || (WRITE && at.block < 0)) return;
-    const unsigned per_head = p.head_dim / 8, half = p.heads * per_head;
-    uint4 x[kUnroll];
-    uint4* to[kUnroll];
+    const int64_t warp = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), token = warp / p.parts;
+    if (token >= p.batch.num_rows) return;
+    const Place at = find_place<WRITE>(p, (int)token);
+    if (at.block == -2) return;
+    const unsigned per_head = p.head_dim / 8, half = p.heads * per_head, all = 2 * half;
+    for (int batch = (int)(warp % p.parts); batch < p.batches; batch += p.parts) {
+        uint4 x[kUnroll];
+        uint4* to[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        unsigned c = (at.part * kUnroll + u) * 32 + (threadIdx.x & 31);
-        to[u] = nullptr;
-        if (c >= 2 * half) continue;
-        const bool is_v = c >= half;
-        c -= is_v ? half : 0;
-        const unsigned head = c / per_head, piece = c % per_head;
-        const RowsView& r = is_v ? p.v : p.k;
-        char* row = r.data + at.token * r.row_stride + head * r.head_stride + piece * 16;
-        char* cached = (is_v ? p.cache.v : p.cache.k) + at.block + (int64_t)head * p.cache.head_stride +
-                       (int64_t)at.offset * p.head_dim * 2 + piece * 16;
-        to[u] = reinterpret_cast<uint4*>(WRITE ? cached : row);
-        x[u] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);       // NaN in both types
-        if (WRITE || at.block >= 0) x[u] = __ldg(reinterpret_cast<const uint4*>(WRITE ? row : cached));
+        for (int u = 0; u < kUnroll; ++u) {
+            unsigned c = (batch * kUnroll + u) * 32 + (threadIdx.x & 31);
+            to[u] = nullptr;
+            if (c >= all) continue;
+            const bool is_v = c >= half;
+            c -= is_v ? half : 0;
+            const unsigned head = c / per_head, piece = c % per_head;
+            const RowsView& r = is_v ? p.v : p.k;
+            char* row = r.data + token * r.row_stride + head * r.head_stride + piece * 16;
+            char* cached = (is_v ? p.cache.v : p.cache.k) + at.block + (int64_t)head * p.cache.head_stride + (int64_t)at.offset * p.head_dim * 2 + piece * 16;
+            to[u] = reinterpret_cast<uint4*>(WRITE ? cached : row);
+            x[u] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);       // NaN in both types
+            if (WRITE || at.block >= 0) x[u] = __ldcs(reinterpret_cast<const uint4*>(WRITE ? row : cached));
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (to[u]) *to[u] = x[u];
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-        if (to[u]) *to[u] = x[u];
 }
 
-// Quantised pools.  A lane has 16 values of a row, a row is a group of `width` lanes (head_dim / 16 rounded up to a
-// power of two) and a warp takes 32 / width rows at a time: the row's largest magnitude needs no shared memory.
+// Quantised pools.  A lane has 16 values of a row in two pieces of 8, a row is a group of `width` lanes (head_dim / 16
+// rounded up to a power of two), so that its largest magnitude needs no shared memory, and a batch is kUnroll rows for
+// each group of lanes.
 template <bool WRITE, bool BF16>
 __global__ void __launch_bounds__(kThreads) kv_cache_move_e4m3(const __grid_constant__ MoveParams p, int width) {
     using H = Half<BF16>;
-    const Place at = find_place<WRITE>(p);
-    if (!at.named || (WRITE && at.block < 0)) return;
-    const int lane = threadIdx.x & 31, sub = lane & (width - 1), rows_at_once = 32 / width;
+    const int64_t warp = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), token = warp / p.parts;
+    if (token >= p.batch.num_rows) return;
+    const Place at = find_place<WRITE>(p, (int)token);
+    if (at.block == -2) return;
+    const int lane = threadIdx.x & 31, sub = lane & (width - 1), group = lane / width, groups = 32 / width;
     const bool active = sub * 16 < p.head_dim;
-#pragma unroll 2
-    for (int u = 0; u < kUnroll; ++u) {
-        int r = (at.part * kUnroll + u) * rows_at_once + lane / width;
-        const bool there = r < 2 * p.heads;
-        if (!__any_sync(0xffffffffu, there)) return;
-        const bool is_v = r >= p.heads;
-        r -= is_v ? p.heads : 0;
-        const RowsView& rows = is_v ? p.v : p.k;
-        uint4* row = reinterpret_cast<uint4*>(rows.data + at.token * rows.row_stride + r * rows.head_stride + sub * 32);
-        char* tile = (is_v ? p.cache.v : p.cache.k) + at.block + (int64_t)r * p.cache.head_stride;
-        uint4* codes = reinterpret_cast<uint4*>(tile + (int64_t)at.offset * p.head_dim + sub * 16);
-        float* scale_at = reinterpret_cast<float*>(tile + (int64_t)p.cache.block_size * p.head_dim) + at.offset;
-        if (WRITE) {
-            uint32_t w[8] = {};
-            if (there && active) {
-                const uint4 a = __ldg(row), b = __ldg(row + 1);
-                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-                w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    const int second = p.head_dim / 2;                              // of the lane's pieces: where it begins, in values
+    const int all = 2 * p.heads;
+    const int64_t scales_at = (int64_t)p.cache.block_size * p.head_dim;
+    for (int batch = (int)(warp % p.parts); batch < p.batches; batch += p.parts) {
+        uint4 a[kUnroll], b[kUnroll];                               // write: the row's pieces; read: a.xy and b.xy, the codes
+        float scale[kUnroll];
+        char *row[kUnroll], *codes[kUnroll];                        // the lane's pieces outside the cache and in it
+        float* scale_at[kUnroll];
+        bool there[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            int r = (batch * kUnroll + u) * groups + group;
+            there[u] = r < all && active;
+            const bool is_v = r >= p.heads;
+            r -= is_v ? p.heads : 0;
+            const RowsView& rows = is_v ? p.v : p.k;
+            row[u] = rows.data + token * rows.row_stride + r * rows.head_stride + sub * 16;
+            char* tile = (is_v ? p.cache.v : p.cache.k) + at.block + (int64_t)r * p.cache.head_stride;
+            codes[u] = tile + (int64_t)at.offset * p.head_dim + sub * 8;
+            scale_at[u] = reinterpret_cast<float*>(tile + scales_at) + at.offset;
+            a[u] = b[u] = make_uint4(0, 0, 0, 0);
+            scale[u] = 0.f;
+            if (WRITE && there[u]) {
+                a[u] = __ldcs(reinterpret_cast<const uint4*>(row[u]));
+                b[u] = __ldcs(reinterpret_cast<const uint4*>(row[u] + second * 2));
+            } else if (there[u] && at.block >= 0) {
+                const uint2 lo = __ldg(reinterpret_cast<const uint2*>(codes[u])), hi = __ldg(reinterpret_cast<const uint2*>(codes[u] + second));
+                a[u].x = lo.x;
+                a[u].y = lo.y;
+                b[u].x = hi.x;
+                b[u].y = hi.y;
+                scale[u] = __ldg(scale_at[u]);
             }
-            uint32_t top = 0;                       // of magnitudes as bit patterns: a NaN is larger than everything
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
-            for (int d = width >> 1; d; d >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
-            top = max(top & 0xffffu, top >> 16);
-            float inverse;
-            const float scale = row_scale<BF16>(top, &inverse);
-            uint32_t out[4];
+        for (int u = 0; u < kUnroll; ++u) {
+            if (WRITE) {
+                const uint32_t w[8] = {a[u].x, a[u].y, a[u].z, a[u].w, b[u].x, b[u].y, b[u].z, b[u].w};
+                uint32_t top = 0;                                   // of magnitudes as bit patterns: a NaN is larger than everything
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 lo = H::to_float2(w[2 * j]), hi = H::to_float2(w[2 * j + 1]);
-                out[j] = encode4(lo.x * inverse, lo.y * inverse, hi.x * inverse, hi.y * inverse);
-            }
-            if (there && active) *codes = make_uint4(out[0], out[1], out[2], out[3]);
-            if (there && sub == 0) *scale_at = scale;
-        } else if (there && active) {
-            uint32_t w[8];
-            if (at.block < 0) {
+                for (int j = 0; j < 8; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+                for (int d = width >> 1; d; d >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
+                top = max(top & 0xffffu, top >> 16);
+                float inverse;
+                const float s = row_scale<BF16>(top, &inverse);
+                uint32_t out[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = H::kNan2;
-            } else {
-                const uint4 c = __ldg(codes);
-                const float scale = __ldg(scale_at), top = H::largest();
-                const uint32_t in[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float2 f = decode2(in[j / 2] >> (j % 2 * 16));
-                    f.x *= scale;
-                    f.y *= scale;
-                    // values beyond the type's largest become that; the comparisons leave a NaN what it is
-                    f.x = f.x > top ? top : f.x < -top ? -top : f.x;
-                    f.y = f.y > top ? top : f.y < -top ? -top : f.y;
-                    w[j] = H::from_float2(f.x, f.y);
+                for (int j = 0; j < 4; ++j) {
+                    const float2 lo = H::to_float2(w[2 * j]), hi = H::to_float2(w[2 * j + 1]);
+                    out[j] = encode4(lo.x * inverse, lo.y * inverse, hi.x * inverse, hi.y * inverse);
                 }
+                if (!there[u]) continue;
+                *reinterpret_cast<uint2*>(codes[u]) = make_uint2(out[0], out[1]);
+                *reinterpret_cast<uint2*>(codes[u] + second) = make_uint2(out[2], out[3]);
+                if (sub == 0) *scale_at[u] = s;
+            } else if (there[u]) {
+                uint4 lo, hi;
+                widen16<BF16>(make_uint4(a[u].x, a[u].y, b[u].x, b[u].y), scale[u], lo, hi);
+                if (at.block < 0) lo = hi = make_uint4(H::kNan2, H::kNan2, H::kNan2, H::kNan2);
+                *reinterpret_cast<uint4*>(row[u]) = lo;
+                *reinterpret_cast<uint4*>(row[u] + second * 2) = hi;
             }
-            row[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            row[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
     }
 }
@@ -238,8 +249,9 @@ int move_rows(const kvmig_rows* k, const kvmig_rows* v, int dtype, void* k_cache
     int width = 1;
     while (width * 16 < head_dim) width *= 2;
     const int64_t pieces = quantised ? 2 * shape->num_heads : 2 * shape->num_heads * head_dim / 8;
-    const int64_t per_warp = kUnroll * (quantised ? 32 / width : 32);
-    p.parts = (int32_t)((pieces + per_warp - 1) / per_warp);
+    const int64_t per_batch = kUnroll * (quantised ? 32 / width : 32);
+    p.batches = (int32_t)((pieces + per_batch - 1) / per_batch);
+    p.parts = (int32_t)std::min<int64_t>(p.batches, std::max<int64_t>(kFillWarps / batch->num_rows, 1));
     const int64_t grid = (batch->num_rows * p.parts + kThreads / 32 - 1) / (kThreads / 32);
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     if (!quantised) kv_cache_move<WRITE><<<(unsigned)grid, kThreads, 0, stream>>>(p);

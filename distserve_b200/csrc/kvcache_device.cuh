@@ -137,4 +137,75 @@ __device__ __forceinline__ float2 decode2(uint32_t codes) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// Pairs of 32-bit floats: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    return x;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(x));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t x;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
+    return x;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t x;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+    return x;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t x;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(a), "l"(b));
+    return x;
+}
+
+// Two e4m3 codes (the low 16 bits) as two 16-bit floats; exact.
+__device__ __forceinline__ uint32_t widen2(uint32_t codes) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 e4m3 codes times their row's scale as 16-bit values: values beyond the type's largest become that.
+template <bool BF16>
+__device__ __forceinline__ void widen16(const uint4& codes, float scale, uint4& lo, uint4& hi) {
+    const uint32_t in[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint32_t out[8];
+    if (!BF16 && scale >= 0x1p-24f && scale <= 128.f) {
+        // the scale is a 16-bit value itself and no product leaves the range
+        const __half2 s = __float2half2_rn(scale);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t w = widen2(in[j / 2] >> (j % 2 * 16));
+            const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&w), s);
+            out[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    } else if (BF16 && scale <= 0x1p100f) {
+        const uint64_t s = pair(scale, scale);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 f = decode2(in[j / 2] >> (j % 2 * 16)), y = unpair(mul_pair(pair(f.x, f.y), s));
+            out[j] = Half<true>::from_float2(y.x, y.y);
+        }
+    } else {
+        using H = Half<BF16>;
+        const float top = H::largest();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float2 f = decode2(in[j / 2] >> (j % 2 * 16));
+            f.x *= scale;
+            f.y *= scale;
+            f.x = f.x > top ? top : f.x < -top ? -top : f.x;
+            f.y = f.y > top ? top : f.y < -top ? -top : f.y;
+            out[j] = H::from_float2(f.x, f.y);
+        }
+    }
+    lo = make_uint4(out[0], out[1], out[2], out[3]);
+    hi = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
 }  // namespace kvmig
