@@ -37,7 +37,7 @@ NVCC_FLAGS = [
 KVMIG_SOURCES = {
     "kvmig": ["kvmig_kernels.cuh"],
     "kvcache": ["kvcache_device.cuh"],
-    "kvattn": ["kvcache_device.cuh", "kvattn_device.cuh", "kvattn_few.cuh", "kvattn_tile.cuh", "tcgen05.cuh"],
+    "kvattn": ["kvcache_device.cuh", "kvattn_device.cuh", "kvattn_few.cuh", "kvattn_load.cuh", "kvattn_tile.cuh", "tcgen05.cuh"],
 }
 SHIM_SOURCES = ["st_pybinding.cpp", "cache_ops.cpp"]
 

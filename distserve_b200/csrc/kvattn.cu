@@ -281,6 +281,8 @@ int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype,
     p.few_tile = (int32_t)plan.few_tile;
     p.block_rows = kBlockRows;
     p.parts = (int32_t)plan.parts;
+    p.few_followed = plan.tiles || plan.parts > 1;
+    p.tiles_followed = plan.parts > 1;
     p.part_out = static_cast<float*>(workspace);
     p.part_stat = reinterpret_cast<float2*>(p.part_out + batch->num_rows * q->num_heads * plan.parts * head_dim);
     return attend(p, &plan, e4m3, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);

@@ -35,6 +35,7 @@ struct AttnParams {
     int32_t box;                       // keys that the copy engine moves at once; 0: it cannot follow this layout
     int32_t q_box;                     // the same for Q: 1 if a tile of 128 rows is one box of tokens x query heads
     int32_t layers, layer;
+    bool few_followed, tiles_followed; // another grid of this call comes after
 };
 
 // Maps of K and V for the copy engine: rows of head_dim values, copied in boxes of 64 values by up to 128 rows.
@@ -73,6 +74,12 @@ __device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, i
 __device__ __forceinline__ int64_t part_keys(int keys, SplitRule rule, int units) {
     const int all = (keys + kSplitKeys - 1) / kSplitKeys;
     return (int64_t)max(max((all + rule.parts - 1) / rule.parts, rule.least), units) * kSplitKeys;
+}
+
+// Lets the next grid of the stream begin.  Only between the grids of one call, which are made for it: another kernel of
+// this library that is allowed to begin early (a migration) must not pass one that reads or writes the pools.
+__device__ __forceinline__ void let_next_begin(bool followed) {
+    if (followed) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attend_few(const __grid_con
     extern __shared__ __align__(128) unsigned char smem[];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, c = lane & 3;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");             // the tile kernel's rows are others
+    let_next_begin(p.few_followed);                        // the tile kernel's rows are others, the join waits
     const int kv_heads = p.heads / p.group, tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
     const int tile = blockIdx.x % tiles, kv_head = blockIdx.x / tiles % kv_heads, seq = blockIdx.x / tiles / kv_heads, split = blockIdx.y;
     const Sequence s = sequence_at(p.batch, seq);

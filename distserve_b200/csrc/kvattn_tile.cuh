@@ -6,21 +6,19 @@
 //   P = 2^(scale S - m), rounded to 16 bits, written back over S's columns;
 //   O += P V    128 x head_dim x 128, P from tensor memory, sums in tensor memory.
 // Each tile has a warpgroup with a thread per row for the softmax, so no value crosses threads.  While one tile's
-// XX a ring of K and V tiles in shared memory: whole tiles through the copy engine, a box per block and 64 values, and
-// what it cannot follow (a sequence's last keys, whose neighbours in the block must become zeros; block sizes that
-// do not tile 128 keys) with cp.async.  Quantised pools pass through a second ring of bytes and are widened to 16 bits
-// by those warps.
+// softmax runs the tensor core works on the other's products.  One warp issues all of them, which keeps the tiles in
+// opposite phases (a warp for each tile lets them fall into step: 150 us instead of 130 for 4096 tokens, 32/4 heads of
+// 128).  The remaining warps fill a ring of K and V tiles in shared memory (kvattn_load.cuh).
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time; until then P may be as large
 // as 256, which costs no precision.  Tensor memory: S0 S1 O0 O1, 128 columns each.
 #pragma once
 
-#include "kvattn_device.cuh"
-#include "tcgen05.cuh"
+#include "kvattn_load.cuh"
 
 namespace kvmig {
 
-constexpr int kTileRows = 128, kTileKeys = 128, kBlockRows = 2 * kTileRows;
+constexpr int kTileRows = 128, kBlockRows = 2 * kTileRows;
 constexpr int kSoftmaxThreads = 256;
 constexpr float kLazy = 8.f;                 // the maximum may lag behind by this many powers of two
 
@@ -36,11 +34,6 @@ template <int HD, bool E4M3> struct TileShape {
     static constexpr int kRing = 2 * kSlot, kRaw = kRing + kSlots * kSlot, kBars = kRaw + kRawSlots * kRawSlot;
     static constexpr int kShared = kBars + kBarriers * 8 + 32 + 1024;       // and room to align the start to 1024
 };
-
-// Byte offset of 16-byte piece j of row r in a tile: columns of 64 values, 128-byte rows, swizzled.
-__device__ __forceinline__ uint32_t tile_offset(int r, int j) {
-    return (uint32_t)((j >> 3) * (kTileKeys * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4));
-}
 
 __device__ unsigned int g_attention_timeouts;      // blocks that gave up waiting
 
@@ -64,7 +57,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
                    drained = pv_done + 16, raw_full = drained + 8, raw_empty = raw_full + T::kRawSlots * 8;
     volatile int* flags = reinterpret_cast<volatile int*>(smem + T::kBars + T::kBarriers * 8);    // failed, bad, tensor memory
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");             // the join waits for the end of this grid
+    let_next_begin(p.tiles_followed);                  // the join waits for the end of this grid
     // Which rows and keys.  Later row tiles, which have more keys, come first.
     const int kv_heads = p.heads / p.group;
     const int tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
@@ -139,7 +132,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, flags[2], 0);
     // A whole warp waits, and goes on or gives up together.
-    auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(bar, parity, flags)) != 0; };
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) { return barrier_wait_warp(bar, parity, flags); };
     // The sign of the scale is taken by the products and a scale of zero by Q, so that the maximum of the scores is theirs too.
     const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
 
@@ -308,177 +301,13 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
             }
         }
         copy_commit();
-        const int count = 2 * steps;                                    // K and V tiles in turn
-        bool bad = false, ok = true;
-        // Whole tiles go through the copy engine where it can follow the layout; the last one of a sequence, whose
-        // missing keys have to be zeros, and other layouts are copied 16 bytes at a time.
-        auto by_engine = [&](int c) { return p.box > 0 && range.begin + (c / 2 + 1) * kTileKeys <= range.end; };
-        // The engine's copies of a paged tile are dealt over the loading warps, one to a lane: box `box_of` of the tile and
-        // its left or right 64 values (codes or scales for quantised pools).  Block ids are read a step ahead.
-        constexpr int kPerBox = E4M3 ? 2 : HD / 64;
-        const int deal = lane * kLoadWarps + w, box_of = deal / kPerBox, part_of = deal % kPerBox;
-        const bool dealt = PAGED && p.box > 0 && box_of < kTileKeys / max(p.box, 1);
-        int ahead = -1;
-        auto look_ahead = [&](int i) {
-            const int key = range.begin + i * kTileKeys + box_of * p.box;
-            ahead = -1;
-            if (dealt && range.begin + (i + 1) * kTileKeys <= range.end && key / p.cache.block_size < p.batch.max_blocks)
-                ahead = p.batch.block_tables[seq * p.batch.table_stride + key / p.cache.block_size];
-        };
-        int id = -1;                                                    // this lane's block in the current step
-        auto engine_block = [&](int c) {
-            if (c % 2 == 0) {
-                id = (unsigned)ahead < (unsigned)p.cache.num_blocks ? ahead : -1;
-                bad |= dealt && id < 0;
-                look_ahead(c / 2 + 1);
-            }
-            return dealt && id >= 0;
-        };
-        if (PAGED) look_ahead(0);
-        // Byte offsets of four keys of a tile, r = lane + 32 x; -1 if there is no such key.
-        int64_t at_k[4], at_v[4];
-        auto look_up = [&](int i) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int key = range.begin + i * kTileKeys + lane + 32 * x;
-                at_k[x] = at_v[x] = -1;
-                if (key >= range.end) continue;
-                if (PAGED) {
-                    const int id = block_of(p.batch, p.cache, seq, key);
-                    if (id < 0) bad = true;
-                    else
-                        at_k[x] = at_v[x] = id * p.cache.block_stride + (int64_t)kv_head * p.cache.head_stride +
-                                            (E4M3 ? (int64_t)(key % p.cache.block_size) << 40 : (int64_t)(key % p.cache.block_size) * HD * 2);
-                } else {
-                    at_k[x] = (int64_t)(s.first + key) * p.k.row_stride + kv_head * p.k.head_stride;
-                    at_v[x] = (int64_t)(s.first + key) * p.v.row_stride + kv_head * p.v.head_stride;
-                }
-            }
-        };
-        auto of_row = [&](int r, bool is_v) {
-            const int64_t mine = r < 32 ? (is_v ? at_v[0] : at_k[0]) : r < 64 ? (is_v ? at_v[1] : at_k[1]) : r < 96 ? (is_v ? at_v[2] : at_k[2]) : (is_v ? at_v[3] : at_k[3]);
-            return mine;
-        };
-        const char* k_data = PAGED ? p.cache.k : p.k.data;
-        const char* v_data = PAGED ? p.cache.v : p.v.data;
-        constexpr int kLag = 2;                                         // tiles in flight behind the newest
-        if constexpr (!E4M3) {
-            for (int c = 0; c < count + kLag; ++c) {
-                if (c < count) {
-                    const int slot = c % T::kSlots;
-                    const uint32_t to = base + T::kRing + slot * T::kSlot;
-                    if (c >= T::kSlots && !(ok = warp_wait(empty(slot), (c / T::kSlots - 1) & 1))) break;
-                    if (by_engine(c)) {
-                        const void* map = c % 2 ? &maps.v : &maps.k;
-                        const int key = range.begin + c / 2 * kTileKeys;
-                        if (!PAGED) {
-                            if (lane == 0) {
-                                if (w > 0) {
-                                    barrier_arrive(full(slot));
-                                } else {
-                                    barrier_expect(full(slot), T::kSlot);
-                                    for (int h = 0; h < HD / 64; ++h) box_copy(to + h * kTileKeys * 128, map, h * 64, kv_head, s.first + key, full(slot));
-                                }
-                            }
-                        } else {
-                            const bool there = engine_block(c);
-                            const int copies = __popc(__ballot_sync(0xffffffffu, there));
-                            if (lane == 0) barrier_expect(full(slot), copies * p.box * 128);
-                            __syncwarp();
-                            if (there)
-                                box_copy(to + part_of * kTileKeys * 128 + box_of * p.box * 128, map, part_of * 64,
-                                         ((id * p.layers + p.layer) * kv_heads + kv_head) * p.cache.block_size + (key + box_of * p.box) % p.cache.block_size, full(slot));
-                        }
-                    } else {
-                        look_up(c / 2);
-                        const char* data = c % 2 ? v_data : k_data;
-                        for (int g = w; g < kTileKeys / kRowsAtOnce; g += kLoadWarps) {
-                            const int r = g * kRowsAtOnce + lane / kPieces, j = lane % kPieces;
-                            const int64_t at = __shfl_sync(0xffffffffu, of_row(g * kRowsAtOnce, c % 2), r & 31);
-                            copy16(to + tile_offset(r, j), data + (at >= 0 ? at + j * 16 : 0), at >= 0);
-                        }
-                    }
-                }
-                copy_commit();
-                if (c >= kLag) {
-                    copy_wait<kLag>();
-                    fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (c == kLag && !(q_by_engine && w == 0)) barrier_arrive(q_full);
-                        if (!by_engine(c - kLag)) barrier_arrive(full((c - kLag) % T::kSlots));
-                    }
-                }
-            }
-        } else {
-            constexpr int kRowPieces = HD / 16, kRawRows = 32 / kRowPieces;
-            auto fetch = [&](int c) {                                   // codes and scales of tile c into the ring of bytes
-                if (c < count && ok) {
-                    const int slot = c % T::kRawSlots;
-                    const uint32_t to = base + T::kRaw + slot * T::kRawSlot;
-                    const char* data = c % 2 ? v_data : k_data;
-                    if (by_engine(c)) {
-                        if (c >= T::kRawSlots && !(ok = warp_wait(raw_empty + slot * 8, (c / T::kRawSlots - 1) & 1))) return;
-                        const bool there = engine_block(c);
-                        const int offset = (range.begin + c / 2 * kTileKeys + box_of * p.box) % p.cache.block_size;
-                        const uint32_t bytes = part_of ? p.box * 4 : p.box * HD, sum = __reduce_add_sync(0xffffffffu, there ? bytes : 0);
-                        if (lane == 0) barrier_expect(raw_full + slot * 8, sum);
-                        __syncwarp();
-                        if (there) {
-                            const char* tile_at = data + id * p.cache.block_stride + (int64_t)kv_head * p.cache.head_stride;
-                            if (part_of)
-                                bulk_copy(to + kTileKeys * HD + box_of * p.box * 4, tile_at + (int64_t)p.cache.block_size * HD + offset * 4, bytes, raw_full + slot * 8);
-                            else
-                                bulk_copy(to + box_of * p.box * HD, tile_at + (int64_t)offset * HD, bytes, raw_full + slot * 8);
-                        }
-                        return;
-                    }
-                    look_up(c / 2);
-                    for (int g = w; g < kTileKeys / kRawRows; g += kLoadWarps) {
-                        const int r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
-                        const int64_t packed = __shfl_sync(0xffffffffu, of_row(g * kRawRows, false), r & 31);
-                        const int64_t tile_at = packed & 0xffffffffffll;
-                        const int offset = (int)(packed >> 40);
-                        const bool there = packed >= 0;
-                        copy16(to + r * HD + j * 16, data + (there ? tile_at + offset * HD + j * 16 : 0), there);
-                        if (j == 0) copy4(to + kTileKeys * HD + r * 4, data + (there ? tile_at + (int64_t)p.cache.block_size * HD + offset * 4 : 0), there);
-                    }
-                }
-            };
-            fetch(0);
-            copy_commit();
-            fetch(1);
-            copy_commit();
-            for (int c = 0; c < count && ok; ++c) {
-                fetch(c + 2);
-                copy_commit();
-                copy_wait<2>();
-                __syncwarp();
-                const int slot = c % T::kSlots, raw_slot = c % T::kRawSlots;
-                if (!ok || (by_engine(c) && !(ok = warp_wait(raw_full + raw_slot * 8, c / T::kRawSlots & 1)))) break;
-                if (c >= T::kSlots && !(ok = warp_wait(empty(slot), (c / T::kSlots - 1) & 1))) break;
-                const unsigned char* raw = smem + T::kRaw + raw_slot * T::kRawSlot;
-                unsigned char* to = smem + T::kRing + slot * T::kSlot;
-#pragma unroll 4
-                for (int g = w; g < kTileKeys / kRawRows; g += kLoadWarps) {
-                    const int r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
-                    uint4 lo, hi;
-                    widen16<BF16>(*reinterpret_cast<const uint4*>(raw + r * HD + j * 16), *reinterpret_cast<const float*>(raw + kTileKeys * HD + r * 4), lo, hi);
-                    const int first = j >= kRowPieces / 2;              // half of the lanes store their second piece first: other banks
-                    *reinterpret_cast<uint4*>(to + tile_offset(r, 2 * j + first)) = first ? hi : lo;
-                    *reinterpret_cast<uint4*>(to + tile_offset(r, 2 * j + 1 - first)) = first ? lo : hi;
-                }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) {
-                    if (c == 0 && !(q_by_engine && w == 0)) barrier_arrive(q_full);      // Q's copies are older than the first tile's
-                    barrier_arrive(raw_empty + raw_slot * 8);
-                    barrier_arrive(full(slot));
-                }
-            }
-        }
-        copy_wait<0>();
-        if (bad) flags[1] = 1;
+        TileLoader<HD, BF16, PAGED, E4M3, kLoadWarps, T::kSlots, T::kRawSlots, true> loader(p, maps, w, seq, kv_head, s.first, range.begin, range.end,
+                                                                                         smem + T::kRing, smem + T::kRaw, full(0), empty(0), raw_full,
+                                                                                         raw_empty, flags);
+        loader.run(2 * steps, [&] {
+            if (lane == 0 && !(q_by_engine && w == 0)) barrier_arrive(q_full);
+        });
+        if (loader.bad) flags[1] = 1;
         __threadfence_block();
         __syncwarp();
         asm volatile("bar.arrive 1, %0;" ::"n"(kSoftmaxThreads + kLoadWarps * 32) : "memory");

@@ -48,6 +48,11 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
     return barrier_wait_slow(bar, parity, failed);
 }
 
+// A whole warp waits, and goes on or gives up together.
+__device__ __forceinline__ bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* failed) {
+    return __all_sync(0xffffffffu, barrier_wait(bar, parity, failed)) != 0;
+}
+
 // Makes this thread's writes to shared memory visible to the tensor core and the copy engine.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
