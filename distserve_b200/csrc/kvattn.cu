@@ -20,7 +20,7 @@ constexpr int64_t kSms = 148;      // of a B200
 // none can have more), the others to the tile kernel; one of the two is launched if the batch can be seen to need only
 // that one.
 struct PagedPlan {
-    bool few, tiles;
+    bool few, tiles, wide;             // wide: blocks of 8 warps instead of 4 for few rows
     int64_t few_rows, few_tile, parts, workspace;
     SplitRule few_rule, tile_rule;
 };
@@ -48,7 +48,12 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
         return SplitRule{(int32_t)std::max<int64_t>(parts, 1), (int32_t)least, (int32_t)blocks};
     };
     plan.few_rule = plan.tile_rule = SplitRule{1, 1, 1};
-    if (plan.few) plan.few_rule = rule(2 * kSms, 4, 4096, b->num_seqs * ((std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile));
+    if (plan.few) {
+        const int64_t tiles = b->num_seqs * ((std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile);
+        plan.few_rule = rule(2 * kSms, 4, 4096, tiles);
+        // short sequences that nobody shares: more warps for each
+        plan.wide = plan.few_rule.parts == 1 && tiles * kv_heads <= kSms;
+    }
     // A block of the tile kernel has an SM to itself; twice as many parts even out sequences of different lengths.
     if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, 4096, b->num_rows * group / kBlockRows + b->num_seqs);
     plan.parts = std::max(plan.few_rule.parts, plan.tile_rule.parts);
@@ -77,14 +82,14 @@ cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-template <int HD, bool BF16, bool E4M3, int MT>
+template <int HD, bool BF16, bool E4M3, int MT, int WARPS>
 int launch_few(const AttnParams& p, cudaStream_t stream, const char* what) {
-    constexpr int smem = FewShape<HD, E4M3, MT>::kShared, rows = FewShape<HD, E4M3, MT>::kRows;
+    constexpr int smem = FewShape<HD, E4M3, MT, WARPS>::kShared, rows = FewShape<HD, E4M3, MT, WARPS>::kRows;
     const int64_t most = std::min((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group, (int64_t)kFewMost);
     const int64_t grid = (int64_t)p.batch.num_seqs * (p.heads / p.group) * std::max<int64_t>((most + rows - 1) / rows, 1);
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many sequences for one call", what);
-    CU_TRY(cudaFuncSetAttribute(attend_few<HD, BF16, E4M3, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attend_few<HD, BF16, E4M3, MT><<<dim3((unsigned)grid, p.few.parts), kFewWarps * 32, smem, stream>>>(p);
+    CU_TRY(cudaFuncSetAttribute(attend_few<HD, BF16, E4M3, MT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attend_few<HD, BF16, E4M3, MT, WARPS><<<dim3((unsigned)grid, p.few.parts), WARPS * 32, smem, stream>>>(p);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
     return 0;
@@ -173,7 +178,8 @@ template <int HD, bool BF16, bool E4M3>
 int launch_paged(const AttnParams& p, const PagedPlan& plan, cudaStream_t stream, const char* what) {
     int rc = 0;
     if (plan.few) {
-        rc = p.few_tile == 16 ? launch_few<HD, BF16, E4M3, 1>(p, stream, what) : launch_few<HD, BF16, E4M3, 2>(p, stream, what);
+        if (plan.wide) rc = p.few_tile == 16 ? launch_few<HD, BF16, E4M3, 1, 8>(p, stream, what) : launch_few<HD, BF16, E4M3, 2, 8>(p, stream, what);
+        else rc = p.few_tile == 16 ? launch_few<HD, BF16, E4M3, 1, 4>(p, stream, what) : launch_few<HD, BF16, E4M3, 2, 4>(p, stream, what);
     }
     if (!rc && plan.tiles) rc = launch_tiles<HD, BF16, true, E4M3>(p, plan.few, stream, what);
     if (rc || p.parts == 1) return rc;

@@ -3,6 +3,8 @@
 // A block takes rows of one sequence that share a KV head, up to 16 or 32 of them (tokens x query heads of the group), and
 // one part of that sequence's keys.  Every K and V value is used for a few rows only, so the kernel is bound by reading
 // the cache; all else is arranged around keeping reads in flight:
+//   * blocks have 4 warps, two blocks to an SM, so that one's start hides behind the other's stream; 8 where whole
+//     sequences leave SMs without a block;
 //   * each warp has its own ring of stages of 16 keys in shared memory, filled by cp.async and drained by that warp
 //     alone: no barrier of the block until the end, and about 96 KiB in flight per SM (two blocks);
 //   * warps take the groups of 16 keys in turn and keep their own running maximum, sum and output, joined at the end;
@@ -16,10 +18,10 @@
 
 namespace kvmig {
 
-constexpr int kFewWarps = 4, kFewKeys = 16;
+constexpr int kFewKeys = 16;
 constexpr int kFewMost = 64;          // rows of a sequence and KV head up to which this kernel is used
 
-template <int HD, bool E4M3, int MT> struct FewShape {
+template <int HD, bool E4M3, int MT, int WARPS> struct FewShape {
     static constexpr int kRows = 16 * MT;
     static constexpr int kRowBytes = HD * (E4M3 ? 1 : 2);
     static constexpr int kTile = kFewKeys * kRowBytes;                          // K or V of one stage
@@ -27,12 +29,12 @@ template <int HD, bool E4M3, int MT> struct FewShape {
     static constexpr int kStages = 24576 / kStage < 8 ? 24576 / kStage : 8;
     static constexpr int kRing = kStages * kStage;
     static constexpr int kJoin = kRows * (HD + 2) * 4;                       // a warp's result, in its own ring
-    static constexpr int kShared = kFewWarps * (kRing > kJoin ? kRing : kJoin);
+    static constexpr int kShared = WARPS * (kRing > kJoin ? kRing : kJoin);
 };
 
-template <int HD, bool BF16, bool E4M3, int MT>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) attend_few(const __grid_constant__ AttnParams p) {
-    using S = FewShape<HD, E4M3, MT>;
+template <int HD, bool BF16, bool E4M3, int MT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid_constant__ AttnParams p) {
+    using S = FewShape<HD, E4M3, MT, WARPS>;
     using H = Half<BF16>;
     constexpr int kSteps = HD / 16;                       // contraction steps of q . k
     constexpr int kChunks = S::kRowBytes / 16;            // 16-byte pieces of a cached row
@@ -47,12 +49,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attend_few(const __grid_con
     const int kv_heads = p.heads / p.group, tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
     const int tile = blockIdx.x % tiles, kv_head = blockIdx.x / tiles % kv_heads, seq = blockIdx.x / tiles / kv_heads, split = blockIdx.y;
     const Sequence s = sequence_at(p.batch, seq);
+    const int tokens = max(p.batch.seq_lens[seq], 0);
     const int64_t total = (int64_t)s.rows * p.group;
     const bool too_many = s.rows > p.batch.max_rows;
     if (total <= (int64_t)tile * S::kRows || total > p.few_rows || (too_many && tile > 0)) return;
     const int row0 = tile * S::kRows;                      // row r of the block: token (row0 + r) / group, query head % group
     const int rows = too_many ? 0 : (int)min(total - row0, (int64_t)S::kRows);
-    const int tokens = max(p.batch.seq_lens[seq], 0), first_pos = tokens - s.rows;   // position of the first token; may be negative
+    const int first_pos = tokens - s.rows;                 // position of the first token; may be negative
     const int len = min(tokens, capacity(p.batch, p.cache));
     int64_t part = part_keys(len, p.few, 0);                                   // keys of a part
     if (part * split < len) part = max(part, part_keys(len, p.few, part_units<false>(p, p.few, S::kRows)));
@@ -110,15 +113,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attend_few(const __grid_con
             }
         }
 
-    unsigned char* ring = smem + warp * (S::kShared / kFewWarps);
+    unsigned char* ring = smem + warp * (S::kShared / WARPS);
     const uint32_t ring_at = shared_address(ring);
     bool bad = too_many || tokens > len;                  // the table is too short for the sequence
 
     // Loading.  Lanes 0..15 each look up one key of the stage to be loaded, one stage ahead of its copies.
     const int64_t head_offset = (int64_t)kv_head * p.cache.head_stride;
     const int groups = (range.end - range.begin + kFewKeys - 1) / kFewKeys;
-    const int mine = groups > warp ? (groups - warp + kFewWarps - 1) / kFewWarps : 0;
-    auto first_key = [&](int i) { return range.begin + (warp + i * kFewWarps) * kFewKeys; };
+    const int mine = groups > warp ? (groups - warp + WARPS - 1) / WARPS : 0;
+    auto first_key = [&](int i) { return range.begin + (warp + i * WARPS) * kFewKeys; };
     auto look_up = [&](int i, int64_t& tile, int& offset) {   // byte offset of the key's tile, -1: nothing to load
         tile = -1;
         offset = 0;
@@ -319,17 +322,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attend_few(const __grid_con
     __syncthreads();
     const int64_t written = too_many ? total : rows;          // all of a sequence's rows become NaN if there are too many
     constexpr int kPairs = HD / 2;
-    for (int64_t x = threadIdx.x; x < written * kPairs; x += kFewWarps * 32) {
+    for (int64_t x = threadIdx.x; x < written * kPairs; x += WARPS * 32) {
         const int64_t r = x / kPairs;
         const int d = (int)(x % kPairs) * 2, in = too_many ? 0 : (int)r;
         float m = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, reinterpret_cast<const float*>(smem + w * (S::kShared / kFewWarps))[in * 2]);
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, reinterpret_cast<const float*>(smem + w * (S::kShared / WARPS))[in * 2]);
         const float base = m == -INFINITY ? 0.f : m;
         float l = 0.f, a = 0.f, b = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) {
-            const float* from = reinterpret_cast<const float*>(smem + w * (S::kShared / kFewWarps));
+        for (int w = 0; w < WARPS; ++w) {
+            const float* from = reinterpret_cast<const float*>(smem + w * (S::kShared / WARPS));
             const float f = exp2_fast(from[in * 2] - base);
             const float2 v = *reinterpret_cast<const float2*>(from + S::kRows * 2 + in * HD + d);
             l += f * from[in * 2 + 1];

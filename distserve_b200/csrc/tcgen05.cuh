@@ -32,6 +32,7 @@ constexpr unsigned long long kWaitNs = 2000000000ull;
 // Waits for a phase, for two seconds at most or until another thread of the block has given up (*failed).
 __device__ __forceinline__ bool barrier_wait_slow(uint32_t bar, uint32_t parity, volatile int* failed) {
     unsigned long long t0, t;
+    if (*failed) return false;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
     for (unsigned i = 0; i < kWaitPolls; ++i) {
         if (barrier_test(bar, parity)) return true;

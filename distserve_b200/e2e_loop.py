@@ -70,6 +70,40 @@ class StandInDecoder:
         torch.matmul(self.weights, self.x, out=self.out)
 
 
+class BatchAttention:
+    """The attention half of a decode step over the requests that have joined the batch: one query token each, every layer
+    of the worker, over the KV that was migrated for them.  The batch's block tables go to the device when the batch
+    changes, not with every step."""
+
+    def __init__(self, worker: KVWorker, query_heads: int, most: int) -> None:
+        self.worker, self.most = worker, most
+        shape = (most, query_heads, worker.model_config.get_head_size())
+        self.q = torch.randn(shape, dtype=worker.model_config.get_torch_dtype(), device=worker.device)
+        self.out = torch.empty_like(self.q)
+        self.requests = []
+        self.tokens = 0                  # attended to, over all layers
+
+    def set_batch(self, requests) -> None:
+        """`requests`: (prompt length, block table) of each, at most `most` of them."""
+        self.requests = requests[-self.most:]
+        n = len(self.requests)
+        if not n:
+            return
+        wide = max(len(blocks) for _, blocks in self.requests)
+        as_ints = lambda x: torch.tensor(x, dtype=torch.int32).to(self.worker.device)  # noqa: E731
+        self.tables = as_ints([list(blocks) + [0] * (wide - len(blocks)) for _, blocks in self.requests])
+        self.lens = as_ints([length for length, _ in self.requests])
+        self.starts = torch.arange(n + 1, dtype=torch.int32, device=self.worker.device)
+
+    def step(self) -> None:
+        n = len(self.requests)
+        if not n:
+            return
+        for layer in range(self.worker.k_cache.shape[1]):
+            self.worker.attend(layer, self.q[:n], self.tables, self.lens, self.starts, 1, out=self.out[:n])
+        self.tokens += self.worker.k_cache.shape[1] * sum(length for length, _ in self.requests)
+
+
 def _arrivals(rate_per_s: float, step_ms: float, steps: int, seed: int) -> List[int]:
     return poisson_arrival_steps(rate_per_s, step_ms, steps, seed)
 
@@ -81,8 +115,10 @@ SIDE_BY_SIDE_OPTIONS = {"chunk_bytes": 32768, "stages": 6, "ctas_per_sm": 1, "ma
 
 
 def run(gpus: int = 1, steps: int = 400, rate: float = 4.0, workload: str = "c5", weight_gb: float = 6.7,
-        pool_blocks: int = 1024, seed: int = 7, time_scale: float = 1.0, overlapped_options: dict = None) -> dict:
-    """`time_scale` > 1 compresses arrival times so that a short run still sees many requests."""
+        pool_blocks: int = 1024, seed: int = 7, time_scale: float = 1.0, overlapped_options: dict = None,
+        attention: bool = False) -> dict:
+    """`time_scale` > 1 compresses arrival times so that a short run still sees many requests.  `attention`: a step also
+    attends, in every layer, over the KV of the requests that have joined the batch."""
     load_ops()
     from . import capi
 
@@ -90,13 +126,13 @@ def run(gpus: int = 1, steps: int = 400, rate: float = 4.0, workload: str = "c5"
     saved = {k: capi.get_option(k) for k in options}
     try:
         with torch.cuda.device(1 if gpus >= 2 else 0):
-            return _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, options, saved)
+            return _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, options, saved, attention)
     finally:
         for k, v in saved.items():
             capi.set_option(k, v)
 
 
-def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, options, defaults) -> dict:
+def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, options, defaults, attention=False) -> dict:
     from . import capi
 
     w = WORKLOADS[workload]
@@ -115,6 +151,7 @@ def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, 
     ctx_worker.v_cache.normal_()
     dec_engine.register_kvcache_mem_handles(pc, handles)
     decoder = StandInDecoder(torch.device("cuda", dec_dev), int(weight_gb * 1e9))
+    attended = BatchAttention(dec_worker, model.num_kv_heads, 64) if attention else None
     compute = torch.cuda.current_stream()
     side = torch.cuda.Stream(device=dec_dev)
 
@@ -145,6 +182,7 @@ def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, 
             for rid in list(bm.block_table):
                 bm.free_blocks(rid)
         pending, lat, blocks, resident = [], [], 0, []
+        joined, stale = set(), True          # requests whose KV is there; the batch on the device is behind them
         nxt = 0
         torch.cuda.synchronize()
         t0 = time.perf_counter()
@@ -157,6 +195,8 @@ def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, 
                         dec_worker.migrate_wait(ticket)
                         lat.append(time.perf_counter() - started_wall[rid])
                         ctx_engine.clear_migrated_blocks(migrating[rid])
+                        joined.add(rid)
+                        stale = True
                     else:
                         still.append((ticket, started, rid))
                 pending = still
@@ -165,6 +205,8 @@ def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, 
                     req = Request.of_length(rid, lens[rid])
                     need = -(-lens[rid] // w.block_size)
                     while dec_engine.block_manager.get_num_avail_gpu_blocks() < need:
+                        joined.discard(resident[0])
+                        stale = True
                         dec_engine.block_manager.free_blocks(resident.pop(0))
                     m = ctx_engine.finish_prefill(req)
                     migrating[rid] = m
@@ -178,6 +220,8 @@ def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, 
                         t1 = time.perf_counter()
                         dec_engine.migrate_blocks(m)              # awaited; frees the context blocks itself
                         lat.append(time.perf_counter() - t1)
+                        joined.add(rid)
+                        stale = True
                     else:
                         dec_engine.block_manager.allocate_blocks(req)
                         target = dec_engine.block_manager.get_block_table(rid)
@@ -186,6 +230,11 @@ def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, 
                         pending.append((ticket, step, rid))
                     nxt += 1
             decoder.step()
+            if attended is not None:
+                if stale:
+                    attended.set_batch([(lens[r], dec_engine.block_manager.get_block_table(r)) for r in resident if r in joined])
+                    stale = False
+                attended.step()
             compute.synchronize()          # a real step returns sampled tokens to the host
         for ticket, _, rid in pending:
             dec_worker.migrate_wait(ticket)
@@ -230,6 +279,7 @@ def _run(gpus, steps, rate, workload, weight_gb, pool_blocks, seed, time_scale, 
         "hidden_fraction": None if added_serial <= 0 else max(0.0, 1.0 - added_overlap / added_serial),
         "p50_migrate_latency_ms": {"serial": ser.p50_latency_ms, "overlapped": ov.p50_latency_ms},
         "overlapped_kernel_options": options,
+        "attended_tokens": attended.tokens if attended is not None else 0,
         "verified": verified,
     }
 
@@ -613,6 +663,7 @@ def run_actors(n_gpus: int = 4, steps: int = 400, rate: float = 4.0, workload: s
 
 def main() -> None:
     ap = argparse.ArgumentParser()
+    ap.add_argument("--attention", action="store_true", help="decode steps also attend over the migrated KV (not with --actors)")
     ap.add_argument("--swap", action="store_true", help="measure swap-out/in beside decode steps instead of migration")
     ap.add_argument("--actors", action="store_true", help="one worker process per GPU, context tp2 -> decoding tp2 per 4 GPUs")
     ap.add_argument("--pool-blocks", type=int, default=1024)
@@ -634,7 +685,7 @@ def main() -> None:
         print(json.dumps(run_actors(args.gpus, args.steps, args.rate, args.workload, args.weight_gb, pool_blocks=args.pool_blocks,
                                     time_scale=args.time_scale, overlapped_options=options, one_shard=args.one_shard)))
         return
-    print(json.dumps(run(args.gpus, args.steps, args.rate, args.workload, args.weight_gb, time_scale=args.time_scale,
+    print(json.dumps(run(args.gpus, args.steps, args.rate, args.workload, args.weight_gb, time_scale=args.time_scale, attention=args.attention,
                          overlapped_options=options)))
 
 
