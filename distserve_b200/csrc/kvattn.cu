@@ -163,12 +163,14 @@ int launch_tiles(const AttnParams& params, bool after_few, cudaStream_t stream, 
     AttnMaps maps = {};
     make_maps(p, maps, PAGED, E4M3, HD, BF16);
     constexpr int smem = TileShape<HD, E4M3>::kShared;
-    const int64_t tiles = ((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group + kBlockRows - 1) / kBlockRows;
-    const int64_t grid = std::max<int64_t>(tiles, 1) * (p.heads / p.group) * p.batch.num_seqs;
+    // Row tiles that there can be, and parts that they can be cut into (part_units).
+    const int64_t kv_heads = p.heads / p.group, tiles = ((int64_t)p.batch.num_rows * p.group / kBlockRows + p.batch.num_seqs) * kv_heads;
+    const int64_t cut = p.tiles.parts > 1 ? std::max<int64_t>(p.tiles.blocks, p.tiles.blocks / 2 + tiles) : tiles;
+    const int64_t grid = (std::min(cut, tiles * p.tiles.parts) + kv_heads - 1) / kv_heads * kv_heads;
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     // After the kernel for few rows, which has other rows to do: begins when that one's blocks leave room.
-    CU_TRY(launch_early(attend_tiles<HD, BF16, PAGED, E4M3>, dim3((unsigned)grid, p.tiles.parts), TileShape<HD, E4M3>::kThreads, smem, after_few,
+    CU_TRY(launch_early(attend_tiles<HD, BF16, PAGED, E4M3>, dim3((unsigned)grid), TileShape<HD, E4M3>::kThreads, smem, after_few,
                         stream, p, maps));
     g_attention_launches++;
     return 0;

@@ -70,10 +70,12 @@ __device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, i
     return (int)fminf((float)sum * kv_heads / blocks, 1e6f) + 1;
 }
 
-// Keys of a part, for a sequence of `keys` of them.
+// Keys of a part, for a sequence of `keys` of them: as few parts as that allows, and those alike.
 __device__ __forceinline__ int64_t part_keys(int keys, SplitRule rule, int units) {
-    const int all = (keys + kSplitKeys - 1) / kSplitKeys;
-    return (int64_t)max(max((all + rule.parts - 1) / rule.parts, rule.least), units) * kSplitKeys;
+    const int all = (keys + kSplitKeys - 1) / kSplitKeys, most = max(max((all + rule.parts - 1) / rule.parts, rule.least), units);
+    if (all <= most) return (int64_t)most * kSplitKeys;
+    const int parts = (all + most - 1) / most;
+    return (int64_t)((all + parts - 1) / parts) * kSplitKeys;
 }
 
 // Lets the next grid of the stream begin.  Only between the grids of one call, which are made for it: another kernel of

@@ -32,7 +32,7 @@ template <int HD, bool E4M3> struct TileShape {
     static constexpr int kRawSlots = E4M3 ? 3 : 0;
     static constexpr int kBarriers = 2 * kSlots + 1 + 8 + 1 + 2 * kRawSlots;
     static constexpr int kRing = 2 * kSlot, kRaw = kRing + kSlots * kSlot, kBars = kRaw + kRawSlots * kRawSlot;
-    static constexpr int kShared = kBars + kBarriers * 8 + 32 + 1024;       // and room to align the start to 1024
+    static constexpr int kShared = kBars + kBarriers * 8 + 64 + 1024;       // and room to align the start to 1024
 };
 
 __device__ unsigned int g_attention_timeouts;      // blocks that gave up waiting
@@ -40,6 +40,86 @@ __device__ unsigned int g_attention_timeouts;      // blocks that gave up waitin
 // The grid may start while the grid before it, which it does not depend on, still runs, but must not end before it:
 // what follows in the stream waits for this one only.
 __device__ __forceinline__ void finish_after_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Row tiles of a sequence (one for a sequence with too many rows, whose rows become NaN; none if it is not this
+// kernel's), and the keys and the number of its parts.
+struct TileWork {
+    int tiles, parts;
+    int64_t part;
+};
+template <bool PAGED>
+__device__ __forceinline__ TileWork work_of(const AttnParams& p, int seq, int units) {
+    TileWork w = {0, 1, INT64_MAX};
+    const Sequence s = sequence_at(p.batch, seq);
+    const int64_t total = (int64_t)s.rows * p.group;
+    if (total == 0 || total <= p.few_rows) return w;
+    if (s.rows > p.batch.max_rows) {
+        w.tiles = 1;
+        return w;
+    }
+    w.tiles = (int)((total + kBlockRows - 1) / kBlockRows);
+    if (PAGED) {
+        const int len = min(max(p.batch.seq_lens[seq], 0), capacity(p.batch, p.cache));
+        w.part = part_keys(len, p.tiles, units);
+        w.parts = max((int)((len + w.part - 1) / w.part), 1);
+    }
+    return w;
+}
+
+// The c-th piece of the call's work for a KV head: a row tile and a part of a sequence's keys.  Long pieces come first:
+// over the cache, sequences with long parts before others; of whole prompts, the last tiles of all of them, which under
+// the causal mask have the most keys, before the first.  (More than 32 sequences, a lane each, are taken in their order.)
+// Nothing is launched for tiles that do not exist, because a block needs an SM to itself even to return.
+template <bool PAGED>
+__device__ __forceinline__ bool find_work(const AttnParams& p, int c, int& seq, int& tile, int& split, int64_t& part) {
+    const int lane = threadIdx.x & 31, n = p.batch.num_seqs, units = PAGED ? part_units<true>(p, p.tiles, kBlockRows) : 0;
+    auto sum = [](int x) { return __reduce_add_sync(0xffffffffu, x); };
+    for (int first = 0; first < n; first += 32) {
+        const TileWork w = first + lane < n ? work_of<PAGED>(p, first + lane, units) : TileWork{0, 1, 0};
+        const int all = sum(w.tiles * w.parts);
+        if (c >= all) {
+            c -= all;
+            continue;
+        }
+        int level = -1, before = 0, mine = w.tiles * w.parts;       // pieces of this lane, and of those that come before it
+        if (PAGED && n <= 32) {
+            const int keys = (int)min(w.part, (int64_t)INT32_MAX);
+            for (int i = 0; i < n; ++i) {
+                const int other = __shfl_sync(0xffffffffu, keys, i), pieces = __shfl_sync(0xffffffffu, mine, i);
+                if (other > keys || (other == keys && i < lane)) before += pieces;
+            }
+        } else {
+            if (n > 1 && n <= 32) {
+                // the largest tile number such that more than c pieces have it or a larger one
+                int high = __reduce_max_sync(0xffffffffu, w.tiles);
+                level = 0;
+                while (level < high) {
+                    const int mid = (level + high + 1) / 2;
+                    if (sum(max(w.tiles - mid, 0) * w.parts) > c) level = mid;
+                    else high = mid - 1;
+                }
+                c -= sum(max(w.tiles - level - 1, 0) * w.parts);
+                mine = w.tiles > level ? w.parts : 0;
+            }
+            before = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, before, d);
+                if (lane >= d) before += x;
+            }
+            before -= mine;
+        }
+        const int owner = __ffs(__ballot_sync(0xffffffffu, c >= before && c < before + mine)) - 1;
+        const int rest = c - __shfl_sync(0xffffffffu, before, owner), parts = __shfl_sync(0xffffffffu, w.parts, owner);
+        seq = first + owner;
+        part = __shfl_sync(0xffffffffu, w.part, owner);
+        split = rest % parts;
+        tile = __shfl_sync(0xffffffffu, w.tiles, owner) - 1 - rest / parts;
+        if (level >= 0) tile = level;
+        return true;
+    }
+    return false;
+}
 
 template <int HD, bool BF16, bool PAGED, bool E4M3>
 __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_tiles(const __grid_constant__ AttnParams p, const __grid_constant__ AttnMaps maps) {
@@ -58,53 +138,30 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
     volatile int* flags = reinterpret_cast<volatile int*>(smem + T::kBars + T::kBarriers * 8);    // failed, bad, tensor memory
 
     let_next_begin(p.tiles_followed);                  // the join waits for the end of this grid
-    // Which rows and keys.  Later row tiles, which have more keys, come first.
-    const int kv_heads = p.heads / p.group;
-    const int tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
-    const int kv_head = blockIdx.x % kv_heads, seq = blockIdx.x / kv_heads % p.batch.num_seqs;
-    const int tile = tiles - 1 - blockIdx.x / (kv_heads * p.batch.num_seqs), split = blockIdx.y;
-    const Sequence s = sequence_at(p.batch, seq);
-    const int64_t total = (int64_t)s.rows * p.group, row0 = (int64_t)tile * kBlockRows;
-    if (row0 >= total || total <= p.few_rows) {        // nothing here, or the other kernel's
-        finish_after_predecessor();
-        return;
-    }
-    if (s.rows > p.batch.max_rows) {                   // more rows than the grid has tiles for
-        if (tile == 0 && split == 0)
-            for (int64_t x = threadIdx.x; x < total * (HD / 8); x += kTileThreads) {
-                const int64_t r = x / (HD / 8);
-                *reinterpret_cast<uint4*>(p.out.data + (s.first + r / p.group) * p.out.row_stride +
-                                          (kv_head * p.group + r % p.group) * p.out.head_stride + x % (HD / 8) * 16) =
-                    make_uint4(H::kNan2, H::kNan2, H::kNan2, H::kNan2);
-            }
-        finish_after_predecessor();
-        return;
-    }
-    const int tokens = PAGED ? max(p.batch.seq_lens[seq], 0) : s.rows, first_pos = tokens - s.rows;
-    const int len = PAGED ? min(tokens, capacity(p.batch, p.cache)) : tokens;
-    int64_t part = len;                                // keys of a part
-    if (PAGED) part = part_keys(len, p.tiles, 0);
-    if (PAGED && part * split < len) part = max(part, part_keys(len, p.tiles, part_units<true>(p, p.tiles, kBlockRows)));
-    if (split > 0 && part * split >= len) {
-        finish_after_predecessor();
-        return;
-    }
-    const bool whole = part >= len;
-    struct { int begin, end; } range = {(int)(part * split), (int)min(part * (split + 1), (int64_t)len)};
-    // Row r of the block is token token0 + (skip + r) / group, query head (skip + r) % group of the group.
-    const int token0 = (int)(row0 / p.group), here = (int)min((int64_t)kBlockRows, total - row0);
-    const unsigned group = p.group, skip = (unsigned)(row0 - (int64_t)token0 * group);
-    int n[2];                                          // key tiles of each row tile
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int end = min((t + 1) * kTileRows, here);
-        const int keys = end <= t * kTileRows ? 0 : (int)min((int64_t)range.end, (int64_t)first_pos + token0 + (skip + end - 1) / group + 1) - range.begin;
-        n[t] = keys > 0 ? (keys + kTileKeys - 1) / kTileKeys : 0;
-    }
-    const int steps = max(n[0], n[1]);
-
+    // Which rows and keys: one warp finds out while others set up.
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
+    const int kv_heads = p.heads / p.group, kv_head = blockIdx.x % kv_heads;
+    volatile int* const work = flags + 3;              // sequence (-1: nothing to do), first row in it, keys [begin, end) and whether they are all
+    if (warp == 0) {
+        int seq = -1, tile = 0, split = 0;
+        int64_t part = 1;
+        const bool any = find_work<PAGED>(p, blockIdx.x / kv_heads, seq, tile, split, part);
+        if (lane == 0) {
+            const Sequence s = sequence_at(p.batch, any ? seq : 0);
+            const int tokens = PAGED ? max(p.batch.seq_lens[any ? seq : 0], 0) : s.rows, len = PAGED ? min(tokens, capacity(p.batch, p.cache)) : tokens;
+            work[0] = any ? seq : -1;
+            work[1] = tile;
+            work[2] = (int)(part * split);
+            work[3] = (int)min(part * (split + 1), (int64_t)len);
+            work[4] = part >= len;
+            work[5] = split;
+            work[6] = s.first;
+            work[7] = s.rows;
+            work[8] = tokens;
+            flags[0] = 0;
+            flags[1] = tokens > len;                   // the table is too short for the sequence
+        }
+    } else if (threadIdx.x == 32) {
         for (int i = 0; i < T::kSlots; ++i) {
             barrier_init(full(i), kLoadWarps);
             barrier_init(empty(i), 1);
@@ -123,13 +180,39 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
-        flags[0] = 0;
-        flags[1] = tokens > len;                       // the table is too short for the sequence
     }
     if (warp == kTileThreads / 32 - 1) tmem_alloc(shared_address(const_cast<int*>(flags + 2)), 512);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
+    struct { int begin, end; } range = {work[2], work[3]};
+    struct { int first, rows; } s = {work[6], work[7]};
+    const int seq = work[0], split = work[5], first_pos = work[8] - s.rows;
+    const bool whole = work[4];
+    const int64_t total = (int64_t)s.rows * p.group, row0 = (int64_t)work[1] * kBlockRows;
+    if (seq < 0 || s.rows > p.batch.max_rows) {
+        if (seq >= 0)
+            for (int64_t x = threadIdx.x; x < total * (HD / 8); x += kTileThreads) {
+                const int64_t r = x / (HD / 8);
+                *reinterpret_cast<uint4*>(p.out.data + (s.first + r / p.group) * p.out.row_stride +
+                                          (kv_head * p.group + r % p.group) * p.out.head_stride + x % (HD / 8) * 16) =
+                    make_uint4(H::kNan2, H::kNan2, H::kNan2, H::kNan2);
+            }
+        if (warp == kTileThreads / 32 - 1) tmem_free(__shfl_sync(0xffffffffu, flags[2], 0), 512);
+        finish_after_predecessor();
+        return;
+    }
+    // Row r of the block is token token0 + (skip + r) / group, query head (skip + r) % group of the group.
+    const int token0 = (int)(row0 / p.group), here = (int)min((int64_t)kBlockRows, total - row0);
+    const unsigned group = p.group, skip = (unsigned)(row0 - (int64_t)token0 * group);
+    int n[2];                                          // key tiles of each row tile
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int end = min((t + 1) * kTileRows, here);
+        const int keys = end <= t * kTileRows ? 0 : (int)min((int64_t)range.end, (int64_t)first_pos + token0 + (skip + end - 1) / group + 1) - range.begin;
+        n[t] = keys > 0 ? (keys + kTileKeys - 1) / kTileKeys : 0;
+    }
+    const int steps = max(n[0], n[1]);
     const uint32_t tmem = __shfl_sync(0xffffffffu, flags[2], 0);
     // A whole warp waits, and goes on or gives up together.
     auto warp_wait = [&](uint32_t bar, uint32_t parity) { return barrier_wait_warp(bar, parity, flags); };
