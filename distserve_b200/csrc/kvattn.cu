@@ -35,27 +35,27 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
     plan.few_rows = !plan.tiles ? INT64_MAX : plan.few ? kFewMost : 0;
     plan.few_tile = most <= 16 ? 16 : 32;
     const int64_t kv_heads = shape->num_heads, head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
-    // A part is at least the call's work over the blocks that the device holds at once (part_units); the device adds the
-    // work up, and the grid has room for the parts of the longest sequence if the others are a quarter as long.  Most of
-    // that room's blocks return at once when there are many sequences, hence the bound by their number; and partial
-    // results stay below 256 MB.
+    // A part is at least the call's work over the blocks that the device holds at once (part_units): the device adds the
+    // work up, the host sees to room for the parts of the longest sequence if the others are a quarter as long, with
+    // partial results below 256 MB.
     const int64_t room = std::max<int64_t>((256 << 20) / std::max<int64_t>(b->num_rows * heads * (head_dim * 4 + 8), 1), 1);
-    auto rule = [&](int64_t blocks, int64_t least, int64_t most_blocks, int64_t row_tiles) {
+    auto rule = [&](int64_t blocks, int64_t least, int64_t row_tiles) {
         const int64_t n = std::max<int64_t>(b->num_seqs, 1), work = row_tiles * kv_heads * units * (n + 3) / (4 * n);
-        const int64_t part = std::max(least, work / blocks + 1), grid = most_blocks / std::max<int64_t>(row_tiles * kv_heads, 1);
+        const int64_t part = std::max(least, work / blocks + 1);
         // joining takes a launch of its own, which two parts of a short sequence are not worth
-        const int64_t parts = units <= 2 * least ? 1 : std::min(std::min((units + part - 1) / part, grid), room);
+        const int64_t parts = units <= 2 * least ? 1 : std::min((units + part - 1) / part, room);
         return SplitRule{(int32_t)std::max<int64_t>(parts, 1), (int32_t)least, (int32_t)blocks};
     };
     plan.few_rule = plan.tile_rule = SplitRule{1, 1, 1};
     if (plan.few) {
         const int64_t tiles = b->num_seqs * ((std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile);
-        plan.few_rule = rule(2 * kSms, 4, 4096, tiles);
+        // beside sequences of the tile kernel there are fewer of this one's than the batch has: as if it were one
+        plan.few_rule = rule(2 * kSms, 4, plan.tiles ? 1 : tiles);
         // short sequences that nobody shares: more warps for each
         plan.wide = plan.few_rule.parts == 1 && tiles * kv_heads <= kSms;
     }
     // A block of the tile kernel has an SM to itself; twice as many parts even out sequences of different lengths.
-    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, 4096, b->num_rows * group / kBlockRows + b->num_seqs);
+    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, b->num_rows * group / kBlockRows + b->num_seqs);
     plan.parts = std::max(plan.few_rule.parts, plan.tile_rule.parts);
     if (plan.parts > 1) plan.workspace = b->num_rows * heads * plan.parts * (head_dim * 4 + (int64_t)sizeof(float2));
     return plan;
@@ -82,14 +82,22 @@ cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
+// Blocks for all the parts that up to `tiles` row tiles can be cut into (see part_units), a multiple of the KV heads.
+int64_t blocks_for(SplitRule rule, int64_t tiles, int64_t kv_heads) {
+    if (rule.parts == 1) return tiles;
+    const int64_t cut = std::max<int64_t>(rule.blocks, rule.blocks / 2 + tiles);
+    return (std::min(cut, tiles * rule.parts) + kv_heads - 1) / kv_heads * kv_heads;
+}
+
 template <int HD, bool BF16, bool E4M3, int MT, int WARPS>
 int launch_few(const AttnParams& p, cudaStream_t stream, const char* what) {
     constexpr int smem = FewShape<HD, E4M3, MT, WARPS>::kShared, rows = FewShape<HD, E4M3, MT, WARPS>::kRows;
     const int64_t most = std::min((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group, (int64_t)kFewMost);
-    const int64_t grid = (int64_t)p.batch.num_seqs * (p.heads / p.group) * std::max<int64_t>((most + rows - 1) / rows, 1);
+    const int64_t kv_heads = p.heads / p.group, tiles = (int64_t)p.batch.num_seqs * kv_heads * std::max<int64_t>((most + rows - 1) / rows, 1);
+    const int64_t grid = blocks_for(p.few, tiles, kv_heads);
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many sequences for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_few<HD, BF16, E4M3, MT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attend_few<HD, BF16, E4M3, MT, WARPS><<<dim3((unsigned)grid, p.few.parts), WARPS * 32, smem, stream>>>(p);
+    attend_few<HD, BF16, E4M3, MT, WARPS><<<(unsigned)grid, WARPS * 32, smem, stream>>>(p);
     CU_TRY(cudaGetLastError());
     g_attention_launches++;
     return 0;
@@ -163,10 +171,8 @@ int launch_tiles(const AttnParams& params, bool after_few, cudaStream_t stream, 
     AttnMaps maps = {};
     make_maps(p, maps, PAGED, E4M3, HD, BF16);
     constexpr int smem = TileShape<HD, E4M3>::kShared;
-    // Row tiles that there can be, and parts that they can be cut into (part_units).
     const int64_t kv_heads = p.heads / p.group, tiles = ((int64_t)p.batch.num_rows * p.group / kBlockRows + p.batch.num_seqs) * kv_heads;
-    const int64_t cut = p.tiles.parts > 1 ? std::max<int64_t>(p.tiles.blocks, p.tiles.blocks / 2 + tiles) : tiles;
-    const int64_t grid = (std::min(cut, tiles * p.tiles.parts) + kv_heads - 1) / kv_heads * kv_heads;
+    const int64_t grid = blocks_for(p.tiles, tiles, kv_heads);
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     // After the kernel for few rows, which has other rows to do: begins when that one's blocks leave room.

@@ -78,6 +78,87 @@ __device__ __forceinline__ int64_t part_keys(int keys, SplitRule rule, int units
     return (int64_t)((all + parts - 1) / parts) * kSplitKeys;
 }
 
+// Row tiles of a sequence (one for a sequence with too many rows, whose rows become NaN; none if it is not the
+// kernel's that asks, see part_units), and the keys and the number of its parts.
+struct TileWork {
+    int tiles, parts;
+    int64_t part;
+};
+template <bool PAGED, bool TILES>
+__device__ __forceinline__ TileWork work_of(const AttnParams& p, SplitRule rule, int tile, int seq, int units) {
+    TileWork w = {0, 1, INT64_MAX};
+    const Sequence s = sequence_at(p.batch, seq);
+    const int64_t total = (int64_t)s.rows * p.group;
+    if (total == 0 || (total > p.few_rows) != TILES) return w;
+    if (s.rows > p.batch.max_rows) {
+        w.tiles = 1;
+        return w;
+    }
+    w.tiles = (int)((total + tile - 1) / tile);
+    if (PAGED) {
+        const int len = min(max(p.batch.seq_lens[seq], 0), capacity(p.batch, p.cache));
+        w.part = part_keys(len, rule, units);
+        w.parts = max((int)((len + w.part - 1) / w.part), 1);
+    }
+    return w;
+}
+
+// The c-th piece of the call's work for a KV head: a row tile and a part of a sequence's keys.  Long pieces come first:
+// over the cache, sequences with long parts before others; of whole prompts, the last tiles of all of them, which under
+// the causal mask have the most keys, before the first.  (More than 32 sequences, a lane each, are taken in their order.)
+// Nothing is launched for pieces that do not exist, because a block needs its shared memory, an SM to itself in the tile
+// kernel, even to return.
+template <bool PAGED, bool TILES>
+__device__ __forceinline__ bool find_work(const AttnParams& p, SplitRule rule, int rows, int c, int& seq, int& tile, int& split, int64_t& part) {
+    const int lane = threadIdx.x & 31, n = p.batch.num_seqs, units = PAGED ? part_units<TILES>(p, rule, rows) : 0;
+    auto sum = [](int x) { return __reduce_add_sync(0xffffffffu, x); };
+    for (int first = 0; first < n; first += 32) {
+        const TileWork w = first + lane < n ? work_of<PAGED, TILES>(p, rule, rows, first + lane, units) : TileWork{0, 1, 0};
+        const int all = sum(w.tiles * w.parts);
+        if (c >= all) {
+            c -= all;
+            continue;
+        }
+        int level = -1, before = 0, mine = w.tiles * w.parts;       // pieces of this lane, and of those that come before it
+        if (PAGED && n <= 32) {
+            const int keys = (int)min(w.part, (int64_t)INT32_MAX);
+            for (int i = 0; i < n; ++i) {
+                const int other = __shfl_sync(0xffffffffu, keys, i), pieces = __shfl_sync(0xffffffffu, mine, i);
+                if (other > keys || (other == keys && i < lane)) before += pieces;
+            }
+        } else {
+            if (n > 1 && n <= 32) {
+                // the largest tile number such that more than c pieces have it or a larger one
+                int high = __reduce_max_sync(0xffffffffu, w.tiles);
+                level = 0;
+                while (level < high) {
+                    const int mid = (level + high + 1) / 2;
+                    if (sum(max(w.tiles - mid, 0) * w.parts) > c) level = mid;
+                    else high = mid - 1;
+                }
+                c -= sum(max(w.tiles - level - 1, 0) * w.parts);
+                mine = w.tiles > level ? w.parts : 0;
+            }
+            before = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, before, d);
+                if (lane >= d) before += x;
+            }
+            before -= mine;
+        }
+        const int owner = __ffs(__ballot_sync(0xffffffffu, c >= before && c < before + mine)) - 1;
+        const int rest = c - __shfl_sync(0xffffffffu, before, owner), parts = __shfl_sync(0xffffffffu, w.parts, owner);
+        seq = first + owner;
+        part = __shfl_sync(0xffffffffu, w.part, owner);
+        split = rest % parts;
+        tile = __shfl_sync(0xffffffffu, w.tiles, owner) - 1 - rest / parts;
+        if (level >= 0) tile = level;
+        return true;
+    }
+    return false;
+}
+
 // Lets the next grid of the stream begin.  Only between the grids of one call, which are made for it: another kernel of
 // this library that is allowed to begin early (a migration) must not pass one that reads or writes the pools.
 __device__ __forceinline__ void let_next_begin(bool followed) {

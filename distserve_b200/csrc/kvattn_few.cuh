@@ -46,8 +46,16 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, c = lane & 3;
     let_next_begin(p.few_followed);                        // the tile kernel's rows are others, the join waits
-    const int kv_heads = p.heads / p.group, tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
-    const int tile = blockIdx.x % tiles, kv_head = blockIdx.x / tiles % kv_heads, seq = blockIdx.x / tiles / kv_heads, split = blockIdx.y;
+    const int kv_heads = p.heads / p.group, kv_head = blockIdx.x % kv_heads;
+    int seq, tile, split = 0;
+    int64_t part = INT64_MAX;                              // keys of a part
+    if (p.few.parts > 1) {
+        if (!find_work<true, false>(p, p.few, S::kRows, blockIdx.x / kv_heads, seq, tile, split, part)) return;
+    } else {                                               // whole sequences: nothing to look for
+        const int tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
+        seq = blockIdx.x / kv_heads % p.batch.num_seqs;
+        tile = tiles - 1 - blockIdx.x / kv_heads / p.batch.num_seqs;
+    }
     const Sequence s = sequence_at(p.batch, seq);
     const int tokens = max(p.batch.seq_lens[seq], 0);
     const int64_t total = (int64_t)s.rows * p.group;
@@ -57,11 +65,9 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
     const int rows = too_many ? 0 : (int)min(total - row0, (int64_t)S::kRows);
     const int first_pos = tokens - s.rows;                 // position of the first token; may be negative
     const int len = min(tokens, capacity(p.batch, p.cache));
-    int64_t part = part_keys(len, p.few, 0);                                   // keys of a part
-    if (part * split < len) part = max(part, part_keys(len, p.few, part_units<false>(p, p.few, S::kRows)));
-    if (split > 0 && part * split >= len) return;
     const bool whole = part >= len;                                            // one part has everything
-    struct { int begin, end; } range = {(int)(part * split), too_many ? 0 : (int)min(part * (split + 1), (int64_t)len)};
+    struct { int begin, end; } range = {(int)(part * split), 0};
+    if (!too_many) range.end = whole ? len : (int)min(part * (split + 1), (int64_t)len);
 
     // Q: lane (quad, c) has rows quad and quad + 8 of each 16.  16-bit pools: step t, values 32 (t/2) + 8 c + 4 (t%2) + 0..3;
     // quantised pools: 64 (t/4) + 16 c + 4 (t%4) + 0..3.
