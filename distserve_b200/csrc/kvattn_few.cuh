@@ -123,7 +123,9 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
     const uint32_t ring_at = shared_address(ring);
     bool bad = too_many || tokens > len;                  // the table is too short for the sequence
 
-    // Loading.  Lanes 0..15 each look up one key of the stage to be loaded, one stage ahead of its copies.
+    // Loading.  Where blocks hold whole groups of 16 keys, the usual case, a group is one run of bytes.  Otherwise lanes
+    // 0..15 each look up one key.  Either is done for the next stage while this one is copied.
+    const bool grouped = p.cache.block_size % kFewKeys == 0;
     const int64_t head_offset = (int64_t)kv_head * p.cache.head_stride;
     const int groups = (range.end - range.begin + kFewKeys - 1) / kFewKeys;
     const int mine = groups > warp ? (groups - warp + WARPS - 1) / WARPS : 0;
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
     auto look_up = [&](int i, int64_t& tile, int& offset) {   // byte offset of the key's tile, -1: nothing to load
         tile = -1;
         offset = 0;
-        const int key = first_key(i) + (lane & 15);
+        const int key = first_key(i) + (grouped ? 0 : lane & 15);
         if (i < mine && key < range.end) {
             const int id = block_of(p.batch, p.cache, seq, key);
             if (id < 0) bad = true;
@@ -145,19 +147,37 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
     auto issue = [&](int i) {
         if (i < mine) {
             const uint32_t at = ring_at + (i % S::kStages) * S::kStage;
+            if (grouped) {
+                const int64_t rows_at = next_tile < 0 ? 0 : next_tile + (int64_t)next_offset * S::kRowBytes;
+                const int count = next_tile < 0 ? 0 : range.end - first_key(i);       // keys that are there, if fewer than 16
+                const char *k_from = p.cache.k + rows_at + lane * 16, *v_from = p.cache.v + rows_at + lane * 16;
 #pragma unroll
-            for (int u = 0; u < kChunks / 2; ++u) {
-                const int piece = u * 32 + lane, r = piece / kChunks, j = piece % kChunks;
-                const int64_t tile = __shfl_sync(0xffffffffu, next_tile, r);
-                const int64_t from = tile + (int64_t)__shfl_sync(0xffffffffu, next_offset, r) * S::kRowBytes + j * 16;
-                const bool valid = tile >= 0;
-                copy16(at + r * S::kRowBytes + ((j ^ ((r & 1) * kFlip)) * 16), p.cache.k + (valid ? from : 0), valid);
-                copy16(at + S::kTile + r * S::kRowBytes + ((j ^ turn(r)) * 16), p.cache.v + (valid ? from : 0), valid);
-            }
-            if (E4M3) {
-                const int64_t tile = __shfl_sync(0xffffffffu, next_tile, lane & 15);
-                const int64_t from = tile + (int64_t)p.cache.block_size * HD + __shfl_sync(0xffffffffu, next_offset, lane & 15) * 4;
-                copy4(at + 2 * S::kTile + lane * 4, (lane < 16 ? p.cache.k : p.cache.v) + (tile >= 0 ? from : 0), tile >= 0);
+                for (int u = 0; u < kChunks / 2; ++u) {
+                    const int piece = u * 32 + lane, r = piece / kChunks, j = piece % kChunks;
+                    const bool valid = r < count;
+                    copy16(at + r * S::kRowBytes + ((j ^ ((r & 1) * kFlip)) * 16), valid ? k_from + u * 512 : p.cache.k, valid);
+                    copy16(at + S::kTile + r * S::kRowBytes + ((j ^ turn(r)) * 16), valid ? v_from + u * 512 : p.cache.v, valid);
+                }
+                if (E4M3) {
+                    const bool valid = (lane & 15) < count;
+                    const int64_t from = next_tile + (int64_t)p.cache.block_size * HD + (next_offset + (lane & 15)) * 4;
+                    copy4(at + 2 * S::kTile + lane * 4, (lane < 16 ? p.cache.k : p.cache.v) + (valid ? from : 0), valid);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < kChunks / 2; ++u) {
+                    const int piece = u * 32 + lane, r = piece / kChunks, j = piece % kChunks;
+                    const int64_t tile = __shfl_sync(0xffffffffu, next_tile, r);
+                    const int64_t from = tile + (int64_t)__shfl_sync(0xffffffffu, next_offset, r) * S::kRowBytes + j * 16;
+                    const bool valid = tile >= 0;
+                    copy16(at + r * S::kRowBytes + ((j ^ ((r & 1) * kFlip)) * 16), p.cache.k + (valid ? from : 0), valid);
+                    copy16(at + S::kTile + r * S::kRowBytes + ((j ^ turn(r)) * 16), p.cache.v + (valid ? from : 0), valid);
+                }
+                if (E4M3) {
+                    const int64_t tile = __shfl_sync(0xffffffffu, next_tile, lane & 15);
+                    const int64_t from = tile + (int64_t)p.cache.block_size * HD + __shfl_sync(0xffffffffu, next_offset, lane & 15) * 4;
+                    copy4(at + 2 * S::kTile + lane * 4, (lane < 16 ? p.cache.k : p.cache.v) + (tile >= 0 ? from : 0), tile >= 0);
+                }
             }
             look_up(i + 1, next_tile, next_offset);
         }
