@@ -44,13 +44,23 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
         const int64_t part = std::max(least, work / blocks + 1);
         // joining takes a launch of its own, which two parts of a short sequence are not worth
         const int64_t parts = units <= 2 * least ? 1 : std::min((units + part - 1) / part, room);
-        return SplitRule{(int32_t)std::max<int64_t>(parts, 1), (int32_t)least, (int32_t)blocks};
+        return SplitRule{(int32_t)std::max<int64_t>(parts, 1), (int32_t)least, (int32_t)blocks, 0};
     };
-    plan.few_rule = plan.tile_rule = SplitRule{1, 1, 1};
+    plan.few_rule = plan.tile_rule = SplitRule{1, 1, 1, 0};
     if (plan.few) {
         const int64_t tiles = b->num_seqs * ((std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile);
         // beside sequences of the tile kernel there are fewer of this one's than the batch has: as if it were one
         plan.few_rule = rule(2 * kSms, 4, plan.tiles ? 1 : tiles);
+        // More row tiles than half of what runs at once: cut so that the last of the waves is full, two extra units being what
+        // a part costs, if that saves a tenth.
+        const int64_t slots = plan.few_rule.blocks, all = tiles * kv_heads;
+        if (!plan.tiles && 2 * all >= slots) {
+            auto cost = [&](int64_t k) { return (double)((all * k + slots - 1) / slots) * ((double)units / k + 2); };
+            int64_t best = 1;
+            for (int64_t k = 2; k <= 8 && units / k >= 4 && 2 * k <= room; ++k)
+                if (cost(k) < 0.9 * cost(1) && cost(k) < cost(best)) best = k;
+            plan.few_rule = SplitRule{best > 1 ? (int32_t)(2 * best) : 1, 4, (int32_t)slots, best > 1 ? (int32_t)best : 0};
+        }
         // short sequences that nobody shares: more warps for each
         plan.wide = plan.few_rule.parts == 1 && tiles * kv_heads <= kSms;
     }
@@ -85,6 +95,7 @@ cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t
 // Blocks for all the parts that up to `tiles` row tiles can be cut into (see part_units), a multiple of the KV heads.
 int64_t blocks_for(SplitRule rule, int64_t tiles, int64_t kv_heads) {
     if (rule.parts == 1) return tiles;
+    if (rule.cuts > 0) return std::min<int64_t>(rule.cuts + 1, rule.parts) * tiles;
     const int64_t cut = std::max<int64_t>(rule.blocks, rule.blocks / 2 + tiles);
     return (std::min(cut, tiles * rule.parts) + kv_heads - 1) / kv_heads * kv_heads;
 }
@@ -324,7 +335,7 @@ int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig
     p.group = (int32_t)(q->num_heads / k->num_heads);
     p.scale_log2 = (float)(scale * 1.4426950408889634);
     p.parts = 1;
-    p.few = p.tiles = SplitRule{1, 1, 1};
+    p.few = p.tiles = SplitRule{1, 1, 1, 0};
     return attend(p, nullptr, false, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
 }
 

@@ -17,6 +17,7 @@ struct AttnRows {
 constexpr int kSplitKeys = 128;
 struct SplitRule {
     int32_t parts, least, blocks;
+    int32_t cuts;      // > 0: a row tile's keys are cut into this many parts on average, whatever fits at once
 };
 
 struct AttnParams {
@@ -45,7 +46,8 @@ struct AttnMaps {
 
 // Units of a part, before `parts` is looked at: from the whole batch's work, which every warp that asks adds up.  TILES:
 // for the sequences of the tile kernel, else for those of the kernel for few rows.  With t row tiles in all, cutting to
-// work / (blocks - t) units leaves no more than `blocks` parts, whatever the lengths.
+// work / (blocks - t) units leaves no more than `blocks` parts, whatever the lengths; cutting to work / (cuts t) units, no
+// more than (cuts + 1) t.
 template <bool TILES>
 __device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, int tile) {
     if (rule.parts == 1) return 0;
@@ -66,6 +68,7 @@ __device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, i
         sum += __shfl_xor_sync(0xffffffffu, sum, d);
         tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
     }
+    if (rule.cuts > 0) return (int)fminf(ceilf((float)sum / ((float)max(tiles, 1u) * rule.cuts)), 1e6f);
     const float blocks = fmaxf((float)rule.blocks - (float)tiles * kv_heads, 0.5f * rule.blocks);
     return (int)fminf((float)sum * kv_heads / blocks, 1e6f) + 1;
 }

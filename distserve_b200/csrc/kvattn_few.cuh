@@ -126,6 +126,8 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
     // Loading.  Where blocks hold whole groups of 16 keys, the usual case, a group is one run of bytes.  Otherwise lanes
     // 0..15 each look up one key.  Either is done for the next stage while this one is copied.
     const bool grouped = p.cache.block_size % kFewKeys == 0;
+    const int shift = (p.cache.block_size & (p.cache.block_size - 1)) == 0 ? 31 - __clz(p.cache.block_size) : -1;
+    const int32_t* const table = p.batch.block_tables + seq * p.batch.table_stride;
     const int64_t head_offset = (int64_t)kv_head * p.cache.head_stride;
     const int groups = (range.end - range.begin + kFewKeys - 1) / kFewKeys;
     const int mine = groups > warp ? (groups - warp + WARPS - 1) / WARPS : 0;
@@ -135,10 +137,11 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
         offset = 0;
         const int key = first_key(i) + (grouped ? 0 : lane & 15);
         if (i < mine && key < range.end) {
-            const int id = block_of(p.batch, p.cache, seq, key);
-            if (id < 0) bad = true;
+            const int entry = shift >= 0 ? key >> shift : key / p.cache.block_size;
+            const int id = entry < p.batch.max_blocks ? table[entry] : -1;
+            if ((unsigned)id >= (unsigned)p.cache.num_blocks) bad = true;
             else tile = id * p.cache.block_stride + head_offset;
-            offset = key % p.cache.block_size;
+            offset = key - entry * p.cache.block_size;
         }
     };
     int64_t next_tile;
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
                     const float* scales = reinterpret_cast<const float*>(ring + (i % S::kStages) * S::kStage + 2 * S::kTile) + n * 8 + 2 * c + e;
                     k_scale[n][e] = scales[0];
                     lift[n][e] = __log2f(scales[16]);
-                    inverse[n][e] = __fdividef(1.f, scales[16]);
+                    inverse[n][e] = scales[16] == 0.f ? 0.f : __fdividef(1.f, scales[16]);    // 0: a key that is not there
                 }
         }
         const bool all = first_key(i) + kFewKeys <= seen_by_all;               // every row sees all of these keys
@@ -280,8 +283,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
                 for (int e = 0; e < 4; ++e) {
                     const float y = exp2_fast(sc[x][n][e] - base[e / 2]);
                     sc[x][n][e] = y;
-                    // a key that is not there may have any scale: it adds nothing
-                    l[x][e / 2] += E4M3 ? (y == 0.f ? 0.f : y * inverse[n][e & 1]) : y;
+                    l[x][e / 2] += E4M3 ? y * inverse[n][e & 1] : y;
                 }
             a[x][0] = In::from_float2(sc[x][0][0], sc[x][0][1]);
             a[x][1] = In::from_float2(sc[x][0][2], sc[x][0][3]);
