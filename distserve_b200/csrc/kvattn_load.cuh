@@ -1,10 +1,10 @@
 // The loading warps of the tensor-core attention kernels: they fill a ring of 128-key tiles, K and V in turn, in the layout
 // that the products read (columns of 64 values, 128-byte rows, swizzled).
 //
-// Whole tiles go through the copy engine, a box for each block and 64 values, or, from quantised pools, as bulk copies of
-// codes and scales into a second ring.  The last tile of a part, whose missing keys have to be zeros (what the
-// pool holds behind a sequence is not read), and block sizes that do not tile 128 keys are copied 16 bytes at a time.
-// Tiles of codes are then widened to 16 bits by these warps.
+// Tiles go through the copy engine, a box for each block and 64 values, or, from quantised pools, as bulk copies of codes
+// and scales into a second ring, whose tiles these warps then widen to 16 bits.  What lies behind the last key of a part
+// comes along with its block, but may be anything: the softmax masks its scores, and its values V are overwritten with
+// zeros here.  Block sizes that do not tile 128 keys are copied 16 bytes at a time, zeros where there is no key.
 #pragma once
 
 #include "kvattn_device.cuh"
@@ -33,45 +33,48 @@ struct TileLoader {
     const AttnMaps& maps;
     const int w, lane, seq, kv_head, first_row, begin, end;
     unsigned char *const ring, *const raw;
-    const uint32_t full, empty, raw_full, raw_empty;
+    const uint32_t full, empty, raw_full, raw_empty, tail;
     volatile int* const flags;
     float* scales = nullptr;
     bool bad = false, ok = true;             // a block that is not there; no wait has run out
 
     // The engine's copies of a paged tile are dealt over the loading warps, one to a lane: box `box_of` of the tile and its
     // left or right 64 values (codes or scales for quantised pools).  Block ids are read a step ahead.
-    int box_of, part_of, id = -1, ahead = -1;
+    int box_of, part_of, id = -2, ahead = -2;    // -2: no copy, -1: no such block
     bool dealt;
     int64_t at_k[4], at_v[4];                // byte offsets of four keys of a tile, r = lane + 32 x; -1 if there is no such key
 
     __device__ __forceinline__ TileLoader(const AttnParams& p_, const AttnMaps& maps_, int w_, int seq_, int kv_head_, int first_row_, int begin_,
                                           int end_, unsigned char* ring_, unsigned char* raw_, uint32_t full_, uint32_t empty_, uint32_t raw_full_,
-                                          uint32_t raw_empty_, volatile int* flags_)
+                                          uint32_t raw_empty_, uint32_t tail_, volatile int* flags_)
         : p(p_), maps(maps_), w(w_), lane(threadIdx.x & 31), seq(seq_), kv_head(kv_head_), first_row(first_row_), begin(begin_), end(end_),
-          ring(ring_), raw(raw_), full(full_), empty(empty_), raw_full(raw_full_), raw_empty(raw_empty_), flags(flags_) {
+          ring(ring_), raw(raw_), full(full_), empty(empty_), raw_full(raw_full_), raw_empty(raw_empty_), tail(tail_), flags(flags_) {
         const int deal = lane * WARPS + w;
         box_of = deal / kPerBox;
         part_of = deal % kPerBox;
         dealt = PAGED && p.box > 0 && box_of < kTileKeys / max(p.box, 1);
     }
 
-    __device__ __forceinline__ bool by_engine(int c) const { return p.box > 0 && begin + (c / 2 + 1) * kTileKeys <= end; }
+    __device__ __forceinline__ bool by_engine() const { return p.box > 0; }
+    __device__ __forceinline__ int keys_of(int c) const { return min(end - begin - c / 2 * kTileKeys, kTileKeys); }     // keys that tile c has
 
     __device__ __forceinline__ void look_ahead(int i) {
         const int key = begin + i * kTileKeys + box_of * p.box;
-        ahead = -1;
-        if (dealt && begin + (i + 1) * kTileKeys <= end && key / p.cache.block_size < p.batch.max_blocks)
-            ahead = p.batch.block_tables[seq * p.batch.table_stride + key / p.cache.block_size];
+        ahead = -2;
+        if (!dealt || key >= end) return;
+        const int entry = key / p.cache.block_size;
+        ahead = entry < p.batch.max_blocks ? p.batch.block_tables[seq * p.batch.table_stride + entry] : -1;
+        if (ahead == -2) ahead = -1;
     }
 
     // This lane's copy of tile c has a source.
     __device__ __forceinline__ bool engine_block(int c) {
         if (c % 2 == 0) {
-            id = (unsigned)ahead < (unsigned)p.cache.num_blocks ? ahead : -1;
-            bad |= dealt && id < 0;
+            id = ahead == -2 || (unsigned)ahead < (unsigned)p.cache.num_blocks ? ahead : -1;
+            bad |= id == -1;
             look_ahead(c / 2 + 1);
         }
-        return dealt && id >= 0;
+        return id >= 0;
     }
 
     __device__ __forceinline__ void look_up(int i) {
@@ -110,9 +113,12 @@ struct TileLoader {
         for (int c = 0; c < count + kLag; ++c) {
             if (c < count) {
                 const int slot = c % SLOTS;
-                const uint32_t to = shared_address(ring) + slot * kSlot, bar = full + slot * 8;
+                const uint32_t to = shared_address(ring) + slot * kSlot;
+                const int keys = keys_of(c);
+                const bool short_v = c % 2 && keys < kTileKeys;
+                const uint32_t bar = short_v && by_engine() ? tail : full + slot * 8;
                 if (c >= SLOTS && !(ok = barrier_wait_warp(empty + slot * 8, (c / SLOTS - 1) & 1, flags))) break;
-                if (by_engine(c)) {
+                if (by_engine()) {
                     const void* map = c % 2 ? &maps.v : &maps.k;
                     const int key = begin + c / 2 * kTileKeys;
                     if (!PAGED) {
@@ -133,6 +139,14 @@ struct TileLoader {
                             box_copy(to + part_of * kTileKeys * 128 + box_of * p.box * 128, map, part_of * 64,
                                      ((id * p.layers + p.layer) * kv_heads + kv_head) * p.cache.block_size + (key + box_of * p.box) % p.cache.block_size, bar);
                     }
+                    if (short_v) {                                            // the last tile: this barrier is used once
+                        ok = barrier_wait_warp(tail, 0, flags);
+                        for (int x = w * 32 + lane; x < (kTileKeys - keys) * kPieces; x += WARPS * 32)
+                            *reinterpret_cast<uint4*>(ring + slot * kSlot + tile_offset(keys + x / kPieces, x % kPieces)) = make_uint4(0, 0, 0, 0);
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) barrier_arrive(full + slot * 8);
+                    }
                 } else {
                     look_up(c / 2);
                     const char* data = PAGED ? (c % 2 ? p.cache.v : p.cache.k) : (c % 2 ? p.v.data : p.k.data);
@@ -149,7 +163,7 @@ struct TileLoader {
                 fence_async_shared();
                 __syncwarp();
                 if (c == kLag) first_loaded();
-                if (lane == 0 && !by_engine(c - kLag)) barrier_arrive(full + (c - kLag) % SLOTS * 8);
+                if (lane == 0 && !by_engine()) barrier_arrive(full + (c - kLag) % SLOTS * 8);
             }
         }
     }
@@ -159,7 +173,7 @@ struct TileLoader {
         const int slot = c % RAW_SLOTS;
         const uint32_t to = shared_address(raw) + slot * kRawSlot, bar = raw_full + slot * 8;
         const char* data = c % 2 ? p.cache.v : p.cache.k;
-        if (by_engine(c)) {
+        if (by_engine()) {
             if (c >= RAW_SLOTS && !(ok = barrier_wait_warp(raw_empty + slot * 8, (c / RAW_SLOTS - 1) & 1, flags))) return;
             const bool there = engine_block(c);
             const int offset = (begin + c / 2 * kTileKeys + box_of * p.box) % p.cache.block_size;
@@ -201,7 +215,7 @@ struct TileLoader {
             copy_wait<kAhead>();
             __syncwarp();
             const int slot = c % SLOTS, raw_slot = c % RAW_SLOTS;
-            if (!ok || (by_engine(c) && !(ok = barrier_wait_warp(raw_full + raw_slot * 8, c / RAW_SLOTS & 1, flags)))) break;
+            if (!ok || (by_engine() && !(ok = barrier_wait_warp(raw_full + raw_slot * 8, c / RAW_SLOTS & 1, flags)))) break;
             const unsigned char* from = raw + raw_slot * kRawSlot;
             uint4 codes[kShare];
             float scale[kShare];
@@ -213,6 +227,7 @@ struct TileLoader {
             }
             if (c >= SLOTS && !(ok = barrier_wait_warp(empty + slot * 8, (c / SLOTS - 1) & 1, flags))) break;
             unsigned char* to = ring + slot * kSlot;
+            const int keys = keys_of(c);
 #pragma unroll
             for (int x = 0; x < kShare; ++x) {
                 const int g = w + x * WARPS, r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
@@ -225,6 +240,7 @@ struct TileLoader {
                     hi = make_uint4(widen2(codes[x].z), widen2(codes[x].z >> 16), widen2(codes[x].w), widen2(codes[x].w >> 16));
                     if (j == 0) scales[slot * kTileKeys + r] = scale[x];
                 }
+                if (c % 2 && r >= keys) lo = hi = make_uint4(0, 0, 0, 0);
                 const bool second = j >= kRowPieces / 2;                  // half of the lanes store their second piece first: other banks
                 *reinterpret_cast<uint4*>(to + tile_offset(r, 2 * j + second)) = second ? hi : lo;
                 *reinterpret_cast<uint4*>(to + tile_offset(r, 2 * j + 1 - second)) = second ? lo : hi;

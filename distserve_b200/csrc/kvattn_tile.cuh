@@ -30,7 +30,7 @@ template <int HD, bool E4M3> struct TileShape {
     static constexpr int kSoftmaxRegisters = E4M3 ? 200 : 208, kOtherRegisters = E4M3 ? 56 : 88;
     static constexpr int kRawSlot = E4M3 ? kTileKeys * (HD + 4) : 0;        // codes, then scales
     static constexpr int kRawSlots = E4M3 ? 3 : 0;
-    static constexpr int kBarriers = 2 * kSlots + 1 + 8 + 1 + 2 * kRawSlots;
+    static constexpr int kBarriers = 2 * kSlots + 1 + 8 + 2 + 2 * kRawSlots;
     static constexpr int kRing = 2 * kSlot, kRaw = kRing + kSlots * kSlot, kBars = kRaw + kRawSlots * kRawSlot;
     static constexpr int kShared = kBars + kBarriers * 8 + 64 + 1024;       // and room to align the start to 1024
 };
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
     auto full = [&](int s) { return bars + s * 8; };
     auto empty = [&](int s) { return bars + (T::kSlots + s) * 8; };
     const uint32_t q_full = bars + 2 * T::kSlots * 8, s_full = q_full + 8, p_half = s_full + 16, p_full = p_half + 16, pv_done = p_full + 16,
-                   drained = pv_done + 16, raw_full = drained + 8, raw_empty = raw_full + T::kRawSlots * 8;
+                   drained = pv_done + 16, tail = drained + 8, raw_full = tail + 8, raw_empty = raw_full + T::kRawSlots * 8;
     volatile int* flags = reinterpret_cast<volatile int*>(smem + T::kBars + T::kBarriers * 8);    // failed, bad, tensor memory
 
     let_next_begin(p.tiles_followed);                  // the join waits for the end of this grid
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
         }
         barrier_init(q_full, kLoadWarps);
         barrier_init(drained, 1);
+        barrier_init(tail, kLoadWarps);
         for (int i = 0; i < T::kRawSlots; ++i) {
             barrier_init(raw_full + i * 8, kLoadWarps);
             barrier_init(raw_empty + i * 8, kLoadWarps);
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
         copy_commit();
         TileLoader<HD, BF16, PAGED, E4M3, kLoadWarps, T::kSlots, T::kRawSlots, true> loader(p, maps, w, seq, kv_head, s.first, range.begin, range.end,
                                                                                          smem + T::kRing, smem + T::kRaw, full(0), empty(0), raw_full,
-                                                                                         raw_empty, flags);
+                                                                                         raw_empty, tail, flags);
         loader.run(2 * steps, [&] {
             if (lane == 0 && !(q_by_engine && w == 0)) barrier_arrive(q_full);
         });
