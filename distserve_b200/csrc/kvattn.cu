@@ -16,7 +16,7 @@ namespace {
 
 constexpr int64_t kSms = 148;      // of a B200
 
-// How a paged call is run.  Sequences with up to kFewMost rows per KV head go to the kernel for few rows (all of them if
+// How a paged call is run.  Sequences with up to few_most() rows per KV head go to the kernel for few rows (all of them if
 // none can have more), the others to the tile kernel; one of the two is launched if the batch can be seen to need only
 // that one.
 struct PagedPlan {
@@ -29,10 +29,11 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
     PagedPlan plan = {};
     const int64_t group = heads / shape->num_heads, most = std::min(b->max_rows, b->num_rows) * group;
     const int64_t capacity = std::min<int64_t>(b->max_blocks * shape->block_size, INT32_MAX), units = (capacity + kSplitKeys - 1) / kSplitKeys;
-    plan.tiles = most > kFewMost;
+    const int64_t bound = few_most(shape->elem_size == 1);
+    plan.tiles = most > bound;
     // rows for every sequence to have its most: as good as certain that all have many
     plan.few = !plan.tiles || b->num_rows < b->num_seqs * b->max_rows;
-    plan.few_rows = !plan.tiles ? INT64_MAX : plan.few ? kFewMost : 0;
+    plan.few_rows = !plan.tiles ? INT64_MAX : plan.few ? bound : 0;
     plan.few_tile = most <= 16 ? 16 : 32;
     const int64_t kv_heads = shape->num_heads, head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
     // A part is at least the call's work over the blocks that the device holds at once (part_units): the device adds the
@@ -40,17 +41,17 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
     // partial results below 256 MB.
     const int64_t room = std::max<int64_t>((256 << 20) / std::max<int64_t>(b->num_rows * heads * (head_dim * 4 + 8), 1), 1);
     auto rule = [&](int64_t blocks, int64_t least, int64_t row_tiles) {
-        const int64_t n = std::max<int64_t>(b->num_seqs, 1), work = row_tiles * kv_heads * units * (n + 3) / (4 * n);
-        const int64_t part = std::max(least, work / blocks + 1);
+        const double n = std::max<int64_t>(b->num_seqs, 1), work = (double)row_tiles * kv_heads * units * (n + 3) / (4 * n);
+        const int64_t part = std::max(least, (int64_t)std::min(work / blocks, (double)units) + 1);
         // joining takes a launch of its own, which two parts of a short sequence are not worth
         const int64_t parts = units <= 2 * least ? 1 : std::min((units + part - 1) / part, room);
         return SplitRule{(int32_t)std::max<int64_t>(parts, 1), (int32_t)least, (int32_t)blocks, 0};
     };
     plan.few_rule = plan.tile_rule = SplitRule{1, 1, 1, 0};
     if (plan.few) {
-        const int64_t tiles = b->num_seqs * ((std::min<int64_t>(most, kFewMost) + plan.few_tile - 1) / plan.few_tile);
+        const int64_t tiles = b->num_seqs * ((std::min(most, bound) + plan.few_tile - 1) / plan.few_tile);
         // beside sequences of the tile kernel there are fewer of this one's than the batch has: as if it were one
-        plan.few_rule = rule(2 * kSms, 4, plan.tiles ? 1 : tiles);
+        plan.few_rule = rule(2 * kSms, 2, plan.tiles ? 1 : tiles);
         // More row tiles than half of what runs at once: cut so that the last of the waves is full, two extra units being what
         // a part costs, if that saves a tenth.
         const int64_t slots = plan.few_rule.blocks, all = tiles * kv_heads;
@@ -103,7 +104,7 @@ int64_t blocks_for(SplitRule rule, int64_t tiles, int64_t kv_heads) {
 template <int HD, bool BF16, bool E4M3, int MT, int WARPS>
 int launch_few(const AttnParams& p, cudaStream_t stream, const char* what) {
     constexpr int smem = FewShape<HD, E4M3, MT, WARPS>::kShared, rows = FewShape<HD, E4M3, MT, WARPS>::kRows;
-    const int64_t most = std::min((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group, (int64_t)kFewMost);
+    const int64_t most = std::min((int64_t)std::min(p.batch.max_rows, p.batch.num_rows) * p.group, p.few_rows);
     const int64_t kv_heads = p.heads / p.group, tiles = (int64_t)p.batch.num_seqs * kv_heads * std::max<int64_t>((most + rows - 1) / rows, 1);
     const int64_t grid = blocks_for(p.few, tiles, kv_heads);
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many sequences for one call", what);

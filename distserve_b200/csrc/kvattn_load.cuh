@@ -37,6 +37,7 @@ struct TileLoader {
     volatile int* const flags;
     float* scales = nullptr;
     bool bad = false, ok = true;             // a block that is not there; no wait has run out
+    int issued = 0;                          // tiles that the copy engine was given
 
     // The engine's copies of a paged tile are dealt over the loading warps, one to a lane: box `box_of` of the tile and its
     // left or right 64 values (codes or scales for quantised pools).  Block ids are read a step ahead.
@@ -105,6 +106,18 @@ struct TileLoader {
         if constexpr (E4M3) run_e4m3(count, first_loaded);
         else run_16(count, first_loaded);
         copy_wait<0>();
+        if (!ok) drain();
+    }
+
+    // A wait has run out: the engine's copies still in flight get a bounded chance to land before their memory is given back.
+    __device__ __forceinline__ void drain() {
+        constexpr int kRing = E4M3 ? RAW_SLOTS : SLOTS;
+        for (int c = max(issued - kRing, 0); c < issued; ++c) {
+            int quiet = 0;
+            const bool short_v = !E4M3 && c % 2 && keys_of(c) < kTileKeys;
+            const uint32_t bar = short_v ? tail : (E4M3 ? raw_full : full) + c % kRing * 8;
+            barrier_wait_warp(bar, short_v ? 0 : c / kRing & 1, &quiet);
+        }
     }
 
     template <typename F>
@@ -119,6 +132,7 @@ struct TileLoader {
                 const uint32_t bar = short_v && by_engine() ? tail : full + slot * 8;
                 if (c >= SLOTS && !(ok = barrier_wait_warp(empty + slot * 8, (c / SLOTS - 1) & 1, flags))) break;
                 if (by_engine()) {
+                    issued = c + 1;
                     const void* map = c % 2 ? &maps.v : &maps.k;
                     const int key = begin + c / 2 * kTileKeys;
                     if (!PAGED) {
@@ -175,6 +189,7 @@ struct TileLoader {
         const char* data = c % 2 ? p.cache.v : p.cache.k;
         if (by_engine()) {
             if (c >= RAW_SLOTS && !(ok = barrier_wait_warp(raw_empty + slot * 8, (c / RAW_SLOTS - 1) & 1, flags))) return;
+            issued = c + 1;
             const bool there = engine_block(c);
             const int offset = (begin + c / 2 * kTileKeys + box_of * p.box) % p.cache.block_size;
             const uint32_t bytes = part_of ? p.box * 4 : p.box * HD, sum = __reduce_add_sync(0xffffffffu, there ? bytes : 0);
