@@ -347,8 +347,8 @@ KVMIG_API int kvmig_cache_read(void* k_cache, void* v_cache, const kvmig_pool_sh
  * h / (q heads / KV heads); the KV heads are the pool's.  head_dim: 64 or 128.
  * scale: finite.  Cached values of the positions that a row's sequence has are
  * finite; what the pool holds elsewhere does not matter.  Scores, softmax and
- * sums are in 32 bits; probabilities are rounded to the 16-bit type for the
- * second product.
+ * sums are in 32 bits; probabilities are rounded to 16 bits for the second
+ * product (to fp16 where the pool is quantised and the rows are few).
  *
  * `workspace` is device memory for the partial results of sequences that are
  * read by several blocks: kvmig_paged_attention_workspace() bytes (0 is a
