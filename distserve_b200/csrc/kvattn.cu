@@ -132,7 +132,10 @@ EncodeTiled encode_tiled() {
 }
 
 // Rows of 16-bit values in boxes of 64 values by [`heads` by] `box` rows, 128-byte swizzle.  dims: values, [heads,] rows.
+// Rows that overlap (a stride of 0, one row standing for all) are not the copy engine's.
 bool encode_map(CUtensorMap* map, const void* data, int rank, const cuuint64_t* dims, const cuuint64_t* strides, int box, bool bf16, int heads = 1) {
+    for (int i = 0; i < rank - 1; ++i)
+        if (strides[i] < dims[0] * 2) return false;
     const cuuint32_t boxes[3] = {64, rank == 3 ? (cuuint32_t)heads : (cuuint32_t)box, (cuuint32_t)box}, steps[3] = {1, 1, 1};
     return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(data), dims,
                           strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

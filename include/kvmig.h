@@ -365,7 +365,8 @@ KVMIG_API int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, 
  * Causal attention of whole packed prompts, before or without a cache: the rows
  * of sequence i attend to the rows of sequence i up to their own.  Of `batch`
  * only num_seqs, num_rows, max_rows and starts are used.  Types, heads,
- * head_dim, scale and arithmetic as above.
+ * head_dim, scale and arithmetic as above; the values of the sequences' rows are
+ * finite, those of rows that no sequence names do not matter.
  */
 KVMIG_API int kvmig_prompt_attention(const kvmig_rows* q, const kvmig_rows* k, const kvmig_rows* v, const kvmig_rows* out,
                                      int dtype, int64_t head_dim, const kvmig_batch* batch, double scale, void* stream);

@@ -198,6 +198,38 @@ def test_prompts(lengths, heads, kv_heads, dim, dtype):
     assert (out[0] == 7).all() and (out[starts[-1]:] == 7).all()
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (8, 2), (5, 1)])
+def test_prompts_with_heads_first_and_with_one_row_for_all(heads, kv_heads):
+    lengths, dim = [150, 1, 300], 64
+    n = sum(lengths)
+    g = torch.Generator().manual_seed(n + heads)
+    q, k, v = (torch.randn(h, n, dim, generator=g).to(torch.bfloat16) for h in (heads, kv_heads, kv_heads))
+    one = lambda t: t[:, 7:8].transpose(0, 1).expand(n, -1, -1)  # noqa: E731
+    first = lambda t: t.transpose(0, 1)  # noqa: E731
+    starts = R.starts_of(lengths)
+    for views in ((first, first, first), (one, first, first), (first, one, first), (first, first, one), (one, one, one)):
+        out = torch.full((heads, n, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+        dq, dk, dv = (view(t.cuda()) for view, t in zip(views, (q, k, v)))
+        torch.ops.kv_attention_ops.prompt(dq, dk, dv, starts.cuda(), max(lengths), 0.125, first(out))
+        hq, hk, hv = (view(t) for view, t in zip(views, (q, k, v)))
+        got = first(out).cpu()
+        for i, (a, b) in enumerate(zip(starts.tolist(), starts.tolist()[1:])):
+            R.assert_close(got[a:b], R.attend(hq[a:b], hk[a:b].double(), hv[a:b].double(), 0.125, "bf16"), f"prompt {i}")
+
+
+@pytest.mark.parametrize("new", [1, 9, 140])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_paged_queries_with_heads_first_and_with_one_row_for_all(new, e4m3):
+    p = R.make_paged(12, [new, new, 2], [60, 700, 3], 2, 128, 16, "fp16", e4m3)
+    q, d = queries(12, 8, 2 * new + 2, 128, "fp16"), p.to("cuda")
+    for view in (lambda t: t.transpose(0, 1), lambda t: t[:, :1].transpose(0, 1).expand(2 * new + 2, -1, -1)):
+        out = torch.full((2 * new + 2, 8, 128), 7.0, dtype=torch.float16, device="cuda")
+        torch.ops.kv_attention_ops.paged(view(q.cuda()), d.k_cache, d.v_cache, d.layer, d.tables, d.lens, d.starts, max(new, 2), 0.09, out)
+        got = out.cpu()
+        for i, e in enumerate(R.attend_paged(p, view(q), 0.09, "fp16")):
+            R.assert_close(got[p.starts[i]:p.starts[i + 1]], e, f"sequence {i}")
+
+
 def test_prompts_do_not_see_each_other_and_too_long_ones_are_nan():
     lengths, dim = [70, 33, 90], 64
     g = torch.Generator().manual_seed(3)
