@@ -25,6 +25,11 @@ struct PagedPlan {
     SplitRule few_rule, tile_rule;
 };
 
+// Row tiles of the tile kernel, of one KV head, that the batch can have.
+int64_t most_tiles(int64_t num_rows, int64_t num_seqs, int64_t max_rows, int64_t group) {
+    return std::min(num_rows * group / kBlockRows + num_seqs, num_seqs * ((std::min(max_rows, num_rows) * group + kBlockRows - 1) / kBlockRows));
+}
+
 PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_batch* b) {
     PagedPlan plan = {};
     const int64_t group = heads / shape->num_heads, most = std::min(b->max_rows, b->num_rows) * group;
@@ -66,9 +71,9 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
         plan.wide = plan.few_rule.parts == 1 && tiles * kv_heads <= kSms;
     }
     // A block of the tile kernel has an SM to itself; twice as many parts even out sequences of different lengths.
-    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, b->num_rows * group / kBlockRows + b->num_seqs);
+    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, most_tiles(b->num_rows, b->num_seqs, b->max_rows, group));
     plan.parts = std::max(plan.few_rule.parts, plan.tile_rule.parts);
-    if (plan.parts > 1) plan.workspace = b->num_rows * heads * plan.parts * (head_dim * 4 + (int64_t)sizeof(float2));
+    if (plan.parts > 1) plan.workspace = b->num_rows * heads * plan.parts * (head_dim * 4 + (int64_t)sizeof(float2)) + 2 * (int64_t)sizeof(int32_t);
     return plan;
 }
 
@@ -186,8 +191,9 @@ int launch_tiles(const AttnParams& params, bool after_few, cudaStream_t stream, 
     AttnMaps maps = {};
     make_maps(p, maps, PAGED, E4M3, HD, BF16);
     constexpr int smem = TileShape<HD, E4M3>::kShared;
-    const int64_t kv_heads = p.heads / p.group, tiles = ((int64_t)p.batch.num_rows * p.group / kBlockRows + p.batch.num_seqs) * kv_heads;
-    const int64_t grid = blocks_for(p.tiles, tiles, kv_heads);
+    const int64_t kv_heads = p.heads / p.group, tiles = std::max<int64_t>(most_tiles(p.batch.num_rows, p.batch.num_seqs, p.batch.max_rows, p.group), p.batch.num_seqs) * kv_heads;
+    const int64_t some = (p.tiles.blocks + kv_heads - 1) / kv_heads * kv_heads;                     // tile_units: no more pieces than this, or tiles
+    const int64_t grid = p.batch.num_seqs > 32 ? blocks_for(p.tiles, tiles, kv_heads) : std::max(tiles, std::min(some, tiles * p.tiles.parts));
     if (grid > INT32_MAX) return fail(KVMIG_ELIMIT, "%s: too many rows for one call", what);
     CU_TRY(cudaFuncSetAttribute(attend_tiles<HD, BF16, PAGED, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     // After the kernel for few rows, which has other rows to do: begins when that one's blocks leave room.
@@ -308,12 +314,12 @@ int kvmig_paged_attention(const kvmig_rows* q, const kvmig_rows* out, int dtype,
     p.few = plan.few_rule;
     p.tiles = plan.tile_rule;
     p.few_tile = (int32_t)plan.few_tile;
-    p.block_rows = kBlockRows;
     p.parts = (int32_t)plan.parts;
     p.few_followed = plan.tiles || plan.parts > 1;
     p.tiles_followed = plan.parts > 1;
     p.part_out = static_cast<float*>(workspace);
     p.part_stat = reinterpret_cast<float2*>(p.part_out + batch->num_rows * q->num_heads * plan.parts * head_dim);
+    p.part_chosen = reinterpret_cast<int32_t*>(p.part_stat + batch->num_rows * q->num_heads * plan.parts);
     return attend(p, &plan, e4m3, head_dim, dtype, batch, static_cast<cudaStream_t>(stream), what);
 }
 

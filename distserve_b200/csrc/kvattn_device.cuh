@@ -29,10 +29,11 @@ struct AttnParams {
     // Sequences of up to few_rows rows per KV head belong to the kernel for few rows, the others to the tile kernel.
     int64_t few_rows;
     SplitRule few, tiles;              // how each cuts a sequence's keys into parts
-    int32_t few_tile, block_rows;      // rows of a block of each
+    int32_t few_tile;                  // rows of a block of the former
     int32_t parts;                     // the parts' partial results, with room for this many:
     float* part_out;                   // [row][head][part][head_dim], sums before the division
     float2* part_stat;                 // [row][head][part]: running maximum (base 2) and sum
+    int32_t* part_chosen;              // units of a part (part_units): few rows, tiles
     int32_t box;                       // keys that the copy engine moves at once; 0: it cannot follow this layout
     int32_t q_box;                     // the same for Q: 1 if a tile of 128 rows is one box of tokens x query heads
     int32_t layers, layer;
@@ -49,7 +50,7 @@ struct AttnMaps {
 // work / (blocks - t) units leaves no more than `blocks` parts, whatever the lengths; cutting to work / (cuts t) units, no
 // more than (cuts + 1) t.
 template <bool TILES>
-__device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, int tile) {
+__device__ __forceinline__ int even_units(const AttnParams& p, SplitRule rule, int tile) {
     if (rule.parts == 1) return 0;
     const int lane = threadIdx.x & 31, room = capacity(p.batch, p.cache), kv_heads = p.heads / p.group;
     unsigned long long sum = 0;
@@ -81,15 +82,77 @@ __device__ __forceinline__ int64_t part_keys(int keys, SplitRule rule, int units
     return (int64_t)((all + parts - 1) / parts) * kSplitKeys;
 }
 
+constexpr int kUncut = 1 << 24;        // units of a part where no sequence is cut
+
+// The same for the tile kernel, whose blocks have an SM each (rule.blocks is two for each): of up to 19 ways to cut, one to a
+// lane, the one that should be over first.  Time is counted in units of kSplitKeys keys; a block's start is worth 3 of
+// them, leaving a partial result and its joining 5 more, the join's launch 3.  Long pieces begin first, so what is expected is
+// the largest of: all work spread evenly, the waves of the longest pieces, and as many waves as there are of the shortest.
+// No more pieces than rule.blocks, or than there are tiles.
+__device__ __forceinline__ int tile_units(const AttnParams& p, SplitRule rule, int tile) {
+    if (rule.parts == 1) return 0;
+    const int lane = threadIdx.x & 31, n = p.batch.num_seqs;
+    if (n > 32) return even_units<true>(p, rule, tile);
+    unsigned units = 0;                                    // of this lane's sequence
+    float count = 0.f;                                     // its row tiles, of all KV heads
+    if (lane < n) {
+        const Sequence s = sequence_at(p.batch, lane);
+        const int64_t total = (int64_t)s.rows * p.group;
+        if (s.rows > 0 && total > p.few_rows) {
+            units = (unsigned)(min(max(p.batch.seq_lens[lane], 0), capacity(p.batch, p.cache)) + kSplitKeys - 1) / kSplitKeys;
+            count = (float)((total + tile - 1) / tile * (p.heads / p.group));
+        }
+    }
+    float work = units * count, tiles = count;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        work += __shfl_xor_sync(0xffffffffu, work, d);
+        tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+    }
+    const unsigned longest = __reduce_max_sync(0xffffffffu, units);
+    const unsigned shortest_part = max((units + rule.parts - 1) / rule.parts, (unsigned)rule.least);      // see part_keys
+    // lanes 0..15: the longest sequence in lane + 1 pieces; 16..18: no more pieces than make one to three waves
+    const float slots = rule.blocks / 2, room = slots * (lane - 15) - tiles;
+    const unsigned unit = lane < 16 ? (longest + lane) / (lane + 1) : (unsigned)fminf(work / fmaxf(room, 1.f), 1e6f) + 1;
+    float all = 0.f, pieces = 0.f, top = 0.f, tops = 0.f, low = 1e9f;
+    bool cut = false;
+    for (int i = 0; i < n; ++i) {
+        const unsigned u = __shfl_sync(0xffffffffu, units, i), most = max(__shfl_sync(0xffffffffu, shortest_part, i), unit);
+        const float c = __shfl_sync(0xffffffffu, count, i);
+        if (c == 0.f) continue;
+        const unsigned parts = u <= most ? 1 : (u + most - 1) / most;
+        const float many = c * parts, piece = parts == 1 ? u + 3 : (u + parts - 1) / parts + 8;
+        cut |= parts > 1;
+        all += many * piece;
+        pieces += many;
+        if (piece >= top) tops = piece == top ? tops + many : many;
+        top = fmaxf(top, piece);
+        low = fminf(low, piece);
+    }
+    float time = fmaxf(all / slots, fmaxf(ceilf(tops / slots) * top, ceilf(pieces / slots) * low)) + (cut ? 3.f : 0.f);
+    if (lane > 18 || (lane > 15 && room <= 0.f) || (lane > 0 && pieces > fmaxf(rule.blocks, tiles))) time = 3e38f;
+    const unsigned best = __reduce_min_sync(0xffffffffu, (__float_as_uint(time) & ~31u) | lane);         // of equals the fewest pieces
+    return __shfl_sync(0xffffffffu, cut, best & 31) ? (int)__shfl_sync(0xffffffffu, unit, best & 31) : kUncut;
+}
+
+// Asked by every block; the first leaves the answer for the join.
+template <bool TILES>
+__device__ __forceinline__ int part_units(const AttnParams& p, SplitRule rule, int tile) {
+    const int units = TILES ? tile_units(p, rule, tile) : even_units<false>(p, rule, tile);
+    if (p.parts > 1 && blockIdx.x == 0 && threadIdx.x == 0) p.part_chosen[TILES] = units;
+    return units;
+}
+
 // Row tiles of a sequence (one for a sequence with too many rows, whose rows become NaN; none if it is not the
 // kernel's that asks, see part_units), and the keys and the number of its parts.
 struct TileWork {
     int tiles, parts;
     int64_t part;
+    int keys;               // of its longest part
 };
 template <bool PAGED, bool TILES>
 __device__ __forceinline__ TileWork work_of(const AttnParams& p, SplitRule rule, int tile, int seq, int units) {
-    TileWork w = {0, 1, INT64_MAX};
+    TileWork w = {0, 1, INT64_MAX, 0};
     const Sequence s = sequence_at(p.batch, seq);
     const int64_t total = (int64_t)s.rows * p.group;
     if (total == 0 || (total > p.few_rows) != TILES) return w;
@@ -102,6 +165,7 @@ __device__ __forceinline__ TileWork work_of(const AttnParams& p, SplitRule rule,
         const int len = min(max(p.batch.seq_lens[seq], 0), capacity(p.batch, p.cache));
         w.part = part_keys(len, rule, units);
         w.parts = max((int)((len + w.part - 1) / w.part), 1);
+        w.keys = (int)min(w.part, (int64_t)len);
     }
     return w;
 }
@@ -112,11 +176,11 @@ __device__ __forceinline__ TileWork work_of(const AttnParams& p, SplitRule rule,
 // Nothing is launched for pieces that do not exist, because a block needs its shared memory, an SM to itself in the tile
 // kernel, even to return.
 template <bool PAGED, bool TILES>
-__device__ __forceinline__ bool find_work(const AttnParams& p, SplitRule rule, int rows, int c, int& seq, int& tile, int& split, int64_t& part) {
-    const int lane = threadIdx.x & 31, n = p.batch.num_seqs, units = PAGED ? part_units<TILES>(p, rule, rows) : 0;
+__device__ __forceinline__ bool find_work(const AttnParams& p, SplitRule rule, int units, int rows, int c, int& seq, int& tile, int& split, int64_t& part) {
+    const int lane = threadIdx.x & 31, n = p.batch.num_seqs;
     auto sum = [](int x) { return __reduce_add_sync(0xffffffffu, x); };
     for (int first = 0; first < n; first += 32) {
-        const TileWork w = first + lane < n ? work_of<PAGED, TILES>(p, rule, rows, first + lane, units) : TileWork{0, 1, 0};
+        const TileWork w = first + lane < n ? work_of<PAGED, TILES>(p, rule, rows, first + lane, units) : TileWork{0, 1, 0, 0};
         const int all = sum(w.tiles * w.parts);
         if (c >= all) {
             c -= all;
@@ -124,7 +188,7 @@ __device__ __forceinline__ bool find_work(const AttnParams& p, SplitRule rule, i
         }
         int level = -1, before = 0, mine = w.tiles * w.parts;       // pieces of this lane, and of those that come before it
         if (PAGED && n <= 32) {
-            const int keys = (int)min(w.part, (int64_t)INT32_MAX);
+            const int keys = w.keys;
             for (int i = 0; i < n; ++i) {
                 const int other = __shfl_sync(0xffffffffu, keys, i), pieces = __shfl_sync(0xffffffffu, mine, i);
                 if (other > keys || (other == keys && i < lane)) before += pieces;

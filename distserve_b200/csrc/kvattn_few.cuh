@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
     int seq, tile, split = 0;
     int64_t part = INT64_MAX;                              // keys of a part
     if (p.few.parts > 1) {
-        if (!find_work<true, false>(p, p.few, S::kRows, blockIdx.x / kv_heads, seq, tile, split, part)) return;
+        if (!find_work<true, false>(p, p.few, part_units<false>(p, p.few, S::kRows), S::kRows, blockIdx.x / kv_heads, seq, tile, split, part)) return;
     } else {                                               // whole sequences: nothing to look for
         const int tiles = gridDim.x / (kv_heads * p.batch.num_seqs);
         seq = blockIdx.x / kv_heads % p.batch.num_seqs;
@@ -396,8 +396,9 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join(const __grid_constan
     constexpr int N = HD / 32;                                // values of a lane
     __shared__ float shared[WIDE ? kJoinWarps * (HD + 2) : 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = WIDE ? warp : 0, step = WIDE ? kJoinWarps : 1;
-    const int few_units = part_units<false>(p, p.few, p.few_tile), tile_units = part_units<true>(p, p.tiles, p.block_rows);
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int few_units = p.few.parts > 1 ? p.part_chosen[0] : kUncut, tile_units = p.tiles.parts > 1 ? p.part_chosen[1] : kUncut;
+    if (few_units == kUncut && tile_units == kUncut) return;
     const int64_t items = (int64_t)p.batch.num_rows * p.heads, stride = (int64_t)gridDim.x * (WIDE ? 1 : kJoinWarps);
     for (int64_t item = (int64_t)blockIdx.x * (WIDE ? 1 : kJoinWarps) + (WIDE ? 0 : warp); item < items; item += stride) {
         const int row = (int)(item / p.heads), head = (int)(item % p.heads);

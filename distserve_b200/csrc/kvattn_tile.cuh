@@ -71,7 +71,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
     if (warp == 0) {
         int seq = -1, tile = 0, split = 0;
         int64_t part = 1;
-        const bool any = find_work<PAGED, true>(p, p.tiles, kBlockRows, blockIdx.x / kv_heads, seq, tile, split, part);
+        const bool any = find_work<PAGED, true>(p, p.tiles, PAGED ? part_units<true>(p, p.tiles, kBlockRows) : 0, kBlockRows, blockIdx.x / kv_heads, seq, tile, split, part);
         if (lane == 0) {
             const Sequence s = sequence_at(p.batch, any ? seq : 0);
             const int tokens = PAGED ? max(p.batch.seq_lens[any ? seq : 0], 0) : s.rows, len = PAGED ? min(tokens, capacity(p.batch, p.cache)) : tokens;
