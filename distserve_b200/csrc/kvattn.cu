@@ -41,7 +41,7 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
     plan.few_rows = !plan.tiles ? INT64_MAX : plan.few ? bound : 0;
     plan.few_tile = most <= 16 ? 16 : 32;
     const int64_t kv_heads = shape->num_heads, head_dim = shape->head_dim - (shape->elem_size == 1 ? KVMIG_SCALE_BYTES : 0);
-    // A part is at least the call's work over the blocks that the device holds at once (part_units): the device adds the
+    // A part is about the call's work over the blocks that the device holds at once (part_units): the device adds the
     // work up, the host sees to room for the parts of the longest sequence if the others are a quarter as long, with
     // partial results below 256 MB.
     const int64_t room = std::max<int64_t>((256 << 20) / std::max<int64_t>(b->num_rows * heads * (head_dim * 4 + 8), 1), 1);
@@ -70,8 +70,11 @@ PagedPlan plan_paged(const kvmig_pool_shape* shape, int64_t heads, const kvmig_b
         // short sequences that nobody shares: more warps for each
         plan.wide = plan.few_rule.parts == 1 && tiles * kv_heads <= kSms;
     }
-    // A block of the tile kernel has an SM to itself; twice as many parts even out sequences of different lengths.
-    if (plan.tiles) plan.tile_rule = rule(2 * kSms, 4, most_tiles(b->num_rows, b->num_seqs, b->max_rows, group));
+    // A block of the tile kernel has an SM to itself; the device chooses how to cut (tile_units).  Up to 2048 keys that is not
+    // worth the choice and the join where the rows fill the SMs anyway (32 sequences of 1032 tokens, 32 of them new, 64/8
+    // heads: 60.7 us, 72.8 with them).
+    if (plan.tiles && (units > 16 || b->num_rows * group / kBlockRows * kv_heads < kSms))
+        plan.tile_rule = rule(2 * kSms, 4, most_tiles(b->num_rows, b->num_seqs, b->max_rows, group));
     plan.parts = std::max(plan.few_rule.parts, plan.tile_rule.parts);
     if (plan.parts > 1) plan.workspace = b->num_rows * heads * plan.parts * (head_dim * 4 + (int64_t)sizeof(float2)) + 2 * (int64_t)sizeof(int32_t);
     return plan;

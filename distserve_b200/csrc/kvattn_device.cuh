@@ -110,6 +110,7 @@ __device__ __forceinline__ int tile_units(const AttnParams& p, SplitRule rule, i
         tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
     }
     const unsigned longest = __reduce_max_sync(0xffffffffu, units);
+    if (longest <= 2 * rule.least) return kUncut;          // joining would cost more than it saves
     const unsigned shortest_part = max((units + rule.parts - 1) / rule.parts, (unsigned)rule.least);      // see part_keys
     // lanes 0..15: the longest sequence in lane + 1 pieces; 16..18: no more pieces than make one to three waves
     const float slots = rule.blocks / 2, room = slots * (lane - 15) - tiles;
@@ -120,9 +121,9 @@ __device__ __forceinline__ int tile_units(const AttnParams& p, SplitRule rule, i
         const unsigned u = __shfl_sync(0xffffffffu, units, i), most = max(__shfl_sync(0xffffffffu, shortest_part, i), unit);
         const float c = __shfl_sync(0xffffffffu, count, i);
         if (c == 0.f) continue;
-        const unsigned parts = u <= most ? 1 : (u + most - 1) / most;
-        const float many = c * parts, piece = parts == 1 ? u + 3 : (u + parts - 1) / parts + 8;
-        cut |= parts > 1;
+        const float parts = u <= most ? 1.f : floorf(__fdividef((float)(u + most) - 0.5f, (float)most)) + (u >> 20 ? 1.f : 0.f);     // exact to 2^20
+        const float many = c * parts, piece = ceilf(__fdividef((float)u, parts)) + (parts > 1.f ? 8.f : 3.f);
+        cut |= parts > 1.f;
         all += many * piece;
         pieces += many;
         if (piece >= top) tops = piece == top ? tops + many : many;

@@ -77,6 +77,16 @@ def test_paged_long_contexts(lengths, heads, kv_heads, dim, dtype, e4m3):
     check_paged(p, queries(heads, sum(new), heads, dim, dtype), dim ** -0.5, dtype)
 
 
+# who is cut: the long one of three; only the one with a single token; one of more sequences than a warp has lanes; nobody
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths", [([300, 260, 70], [6000, 200, 0]), ([1, 130], [6000, 300]), ([70] * 34, [0] * 20 + [5000] + [30] * 13),
+                                     ([70] * 40, [1100] * 40), ([200, 1, 200], [2300, 2300, 2300])], ids=["long", "single", "many", "none", "alike"])
+def test_keys_are_cut_unevenly(lengths, e4m3):
+    new, ctx = lengths
+    p = R.make_paged(21, new, ctx, 2, 64, 16, "bf16", e4m3)
+    check_paged(p, queries(21, sum(new), 4, 64, "bf16"), 0.125, "bf16")
+
+
 @pytest.mark.parametrize("new", [[1, 1], [6, 6], [40, 40]], ids=str)
 @pytest.mark.parametrize("scale,magnitude", [(0.0, 1.0), (-0.3, 1.0), (1.0, 8.0), (0.088, 1e-4), (0.088, 40.0)])
 def test_paged_scales_and_magnitudes(scale, magnitude, new):
