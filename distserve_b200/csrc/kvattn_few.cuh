@@ -23,8 +23,8 @@ namespace kvmig {
 
 constexpr int kFewKeys = 16;
 // Rows of a sequence and KV head up to which this kernel is used.  Beyond 32 it reads the cache twice, which the tile kernel
-// beats on 16-bit pools (8 sequences of 4000 tokens, 48 rows: 38.5 us against 41.6) but not where it has to widen codes for
-// tiles of 256 rows (52.5 against 43.4); at 96 rows it wins on both (40.5 against 65.6, 54.1 against 70.1).
+// beats on 16-bit pools (8 sequences of 4000 tokens, 16 KV heads: 32 rows 73 us here and 76 there, 48 rows 109 and 77) but not
+// where it has to widen codes for tiles of 256 rows (64 rows 122 and 147, 96 rows 204 and 146).
 constexpr int few_most(bool e4m3) { return e4m3 ? 64 : 32; }
 
 template <int HD, bool E4M3, int MT, int WARPS> struct FewShape {

@@ -10,7 +10,8 @@
  * The functions replace the four native operators that DistServe resolves from
  * SwiftTransformer's libst_pybinding.so (distserve/__init__.py:4-16).  The
  * operator shim in libst_pybinding.so (same directory as this library) binds
- * them under the operator names the reference calls.
+ * them under the operator names the reference calls.  What writes, reads and
+ * attends over the cache's contents (further below) has no counterpart there.
  *
  * Pool layout, both stages, K and V separately (distserve/worker.py:107-121):
  *   [num_blocks, layers_local, kv_heads_local, block_size, head_dim], contiguous.
