@@ -11,7 +11,10 @@
 //   * products run on m16n8k16 matrix instructions with the rows padded to 16 or 32.  Contraction order is free, so K
 //     fragments are read as 16 consecutive bytes per lane and Q's values are permuted to match, once;
 //   * e4m3 codes widen to 16 bits in registers; K's scales multiply the scores.  V's scale s_j goes into the exponent,
-//     P_j = 2^(score_j + log2 s_j - m), and the sum counts P_j / s_j: nothing can leave the 16-bit range that way.
+//     P_j = 2^(score_j + log2 s_j - m + 15), so that no P_j leaves fp16 at the upper end, and the sum counts P_j / s_j.  At the
+//     lower end fp16 holds P_j to eleven bits down to 2^-29 of its largest value and to 2^-40 of it below.  A row's scale is the
+//     size of its values, so that is what a value weighs in the output, but for a row of zeros, whose scale is 1 whatever
+//     its neighbours' are: one that would raise m counts with kZeroRowScale instead, or it would push the others out of the range.
 // Measured: 64 requests with 40 heads of 128, 41k cached tokens, 838 MB: 138 us (6.1 TB/s, 95% of a copy); 32 requests of
 // 2000 tokens, 16 heads: 83 us from 16 bits (6.3 TB/s), 74 us from e4m3 (3.7 TB/s: instructions per byte, a third of them
 // widening, are what bounds it; a third block per SM with a smaller ring gained nothing).
@@ -26,6 +29,14 @@ constexpr int kFewKeys = 16;
 // beats on 16-bit pools (8 sequences of 4000 tokens, 16 KV heads: 32 rows 73 us here and 76 there, 48 rows 109 and 77) but not
 // where it has to widen codes for tiles of 256 rows (64 rows 122 and 147, 96 rows 204 and 146).
 constexpr int few_most(bool e4m3) { return e4m3 ? 64 : 32; }
+
+// Quantised pools: P_j's largest value is 2^15 (kTopLog2).  The sum counts P_j 2^-6 / s_j (kSumUnit), since 1 / s_j alone reaches
+// 2^100 and 2^-120: neither that nor the sum of 2^18 keys leaves the range of 32 bits.
+constexpr float kTopLog2 = 15.f, kTop = 0x1p15f, kSumUnit = 0x1p-6f;
+// The scale that a V row of zeros counts with where it would raise the maximum: 2^-64.  Below those of the other rows it leaves
+// P_j its range; and weights down to 2^-24 are in the sum while scales differ by less than 2^117.  So zeros go with any V of
+// fp16 rows (scales 2^-32 .. 2^8), and with bf16 rows of 2^-70 .. 2^60.
+constexpr float kZeroRowLog2 = -64.f, kZeroRowScale = 0x1p-64f;
 
 template <int HD, bool E4M3, int MT, int WARPS> struct FewShape {
     static constexpr int kRows = 16 * MT;
@@ -237,23 +248,43 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
             }
         }
         const int key = first_key(i) + 2 * c;
-        float k_scale[2][2], lift[2][2], inverse[2][2];        // K's scale, log2 and inverse of V's scale
+        float* const scales = reinterpret_cast<float*>(ring + (i % S::kStages) * S::kStage + 2 * S::kTile);     // K's, then V's
+        float k_scale[2][2], lift[2][2];                       // K's scale, log2 of V's
         if (E4M3) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float* scales = reinterpret_cast<const float*>(ring + (i % S::kStages) * S::kStage + 2 * S::kTile) + n * 8 + 2 * c + e;
-                    k_scale[n][e] = scales[0];
-                    lift[n][e] = __log2f(scales[16]);
-                    inverse[n][e] = scales[16] == 0.f ? 0.f : __fdividef(1.f, scales[16]);    // 0: a key that is not there
+                    k_scale[n][e] = scales[n * 8 + 2 * c + e];
+                    lift[n][e] = __log2f(scales[kFewKeys + n * 8 + 2 * c + e]);
                 }
         }
-        const bool all = first_key(i) + kFewKeys <= seen_by_all;               // every row sees all of these keys
-        uint32_t a[MT][4];
+        float inverse[2][2];                                   // of V's scale
+        auto find_inverse = [&] {
 #pragma unroll
-        for (int x = 0; x < MT; ++x) {
-            float top[2] = {m[x][0], m[x][1]};
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float scale = scales[kFewKeys + n * 8 + 2 * c + e];
+                    inverse[n][e] = scale == 0.f ? 0.f : __fdividef(kSumUnit, scale);              // 0: a key that is not there
+                }
+        };
+        // With 16 rows early enough not to be waited for (32 x 2000 tokens: 3% faster); 32 have no registers to keep it in (4% slower).
+        if (E4M3 && MT == 1) find_inverse();
+        const bool all = first_key(i) + kFewKeys <= seen_by_all;               // every row sees all of these keys
+        float top[MT][2];
+        auto find_top = [&] {
+#pragma unroll
+            for (int x = 0; x < MT; ++x)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    top[x][h] = fmaxf(fmaxf(m[x][h], fmaxf(sc[x][0][2 * h], sc[x][0][2 * h + 1])), fmaxf(sc[x][1][2 * h], sc[x][1][2 * h + 1]));
+#pragma unroll
+                    for (int d = 1; d < 4; d <<= 1) top[x][h] = fmaxf(top[x][h], __shfl_xor_sync(0xffffffffu, top[x][h], d));
+                }
+        };
+#pragma unroll
+        for (int x = 0; x < MT; ++x)
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -263,18 +294,45 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
                     const int at = key + n * 8 + (e & 1);
                     if (!all) y = at <= last[x][e / 2] && at < range.end ? y : -INFINITY;
                     sc[x][n][e] = y;
-                    top[e / 2] = fmaxf(top[e / 2], y);
                 }
+        find_top();
+        bool grown = false;
 #pragma unroll
-            for (int d = 1; d < 4; d <<= 1)
+        for (int x = 0; x < MT; ++x) grown |= top[x][0] > m[x][0] || top[x][1] > m[x][1];
+        if (__any_sync(0xffffffffu, grown)) {
+            if (E4M3 && __any_sync(0xffffffffu, scales[kFewKeys + (lane & 15)] == 1.f)) {
+                // Whose rows of V are zeros?  A lane looks at half of key (lane & 15)'s.
+                uint32_t codes = 0;
+#pragma unroll 1
+                for (int u = 0; u < kChunks / 2; ++u) {
+                    const uint4 w = load_shared16(v_at + (lane & 15) * S::kRowBytes + (lane >> 4) * (S::kRowBytes / 2) + u * 16);
+                    codes |= w.x | w.y | w.z | w.w;
+                }
+                uint32_t zeros = __ballot_sync(0xffffffffu, scales[kFewKeys + (lane & 15)] == 1.f && (codes & 0x7f7f7f7fu) == 0);
+                zeros &= zeros >> 16;
+                if (zeros >> lane & 1) scales[kFewKeys + lane] = kZeroRowScale;
+                __syncwarp();
 #pragma unroll
-                for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
-            if (__any_sync(0xffffffffu, top[0] > m[x][0] || top[1] > m[x][1])) {
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (zeros >> (n * 8 + 2 * c + e) & 1) {
+#pragma unroll
+                            for (int x = 0; x < MT; ++x) {
+                                sc[x][n][e] += kZeroRowLog2;
+                                sc[x][n][e + 2] += kZeroRowLog2;
+                            }
+                        }
+                find_top();
+                if (MT == 1) find_inverse();
+            }
+#pragma unroll
+            for (int x = 0; x < MT; ++x) {
                 float keep[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    keep[h] = m[x][h] == top[h] ? 1.f : exp2_fast(m[x][h] - top[h]);
-                    m[x][h] = top[h];
+                    keep[h] = m[x][h] == top[x][h] ? 1.f : exp2_fast(m[x][h] - top[x][h]);
+                    m[x][h] = top[x][h];
                     l[x][h] *= keep[h];
                 }
 #pragma unroll
@@ -282,7 +340,13 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[x][n][e] *= keep[e / 2];
             }
-            const float base[2] = {m[x][0] == -INFINITY ? 0.f : m[x][0], m[x][1] == -INFINITY ? 0.f : m[x][1]};   // a row without a key yet
+        }
+        if (E4M3 && MT > 1) find_inverse();
+        uint32_t a[MT][4];
+#pragma unroll
+        for (int x = 0; x < MT; ++x) {
+            constexpr float top_log2 = E4M3 ? kTopLog2 : 0.f;
+            const float base[2] = {m[x][0] == -INFINITY ? 0.f : m[x][0] - top_log2, m[x][1] == -INFINITY ? 0.f : m[x][1] - top_log2};   // a row without a key yet
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -329,6 +393,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int d = 1; d < 4; d <<= 1) l[x][h] += __shfl_xor_sync(0xffffffffu, l[x][h], d);
+            if (E4M3) l[x][h] *= 1.f / (kTop * kSumUnit);
             if (bad) l[x][h] = not_a_number();
         }
 
@@ -349,8 +414,9 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
             for (int n = 0; n < HD / 8; ++n) {
                 // columns of the lane's values: 8 n + 2 c + {0, 1}, or of the even/odd tiles 16 (n/2) + 4 c + n%2 + {0, 2}
                 const int d = E4M3 ? 16 * (n / 2) + 4 * c + n % 2 : 8 * n + 2 * c, step = E4M3 ? 2 : 1;
-                out[r * HD + d] = o[x][n][2 * h];
-                out[r * HD + d + step] = o[x][n][2 * h + 1];
+                constexpr float down = E4M3 ? 1.f / kTop : 1.f;
+                out[r * HD + d] = o[x][n][2 * h] * down;
+                out[r * HD + d + step] = o[x][n][2 * h + 1] * down;
             }
         }
     __syncthreads();

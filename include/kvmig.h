@@ -348,8 +348,15 @@ KVMIG_API int kvmig_cache_read(void* k_cache, void* v_cache, const kvmig_pool_sh
  * h / (q heads / KV heads); the KV heads are the pool's.  head_dim: 64 or 128.
  * scale: finite.  Cached values of the positions that a row's sequence has are
  * finite; what the pool holds elsewhere does not matter.  Scores, softmax and
- * sums are in 32 bits; probabilities are rounded to 16 bits for the second
- * product (to fp16 where the pool is quantised and the rows are few).
+ * sums are in 32 bits; probabilities are rounded to the rows' 16-bit type for
+ * the second product.  Over quantised pools, a sequence of at most 64 rows per
+ * KV head may have its probabilities rounded together with V's scales, p_j s_j,
+ * in fp16: to 2^-11 of themselves, or to 2^-40 of their largest where they are
+ * below 2^-29 of it.  (A V row of zeros, whatever its scale, draws its weight
+ * and takes no precision from the others, whose largest magnitudes have to be
+ * within 2^-70 .. 2^60 for that; without such rows, within 2^117 of each
+ * other.)  Otherwise K and V are widened to the rows' type first: values
+ * beyond its largest become that.
  *
  * `workspace` is device memory for the partial results of sequences that are
  * read by several blocks: kvmig_paged_attention_workspace() bytes (0 is a
