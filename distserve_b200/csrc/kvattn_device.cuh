@@ -45,24 +45,34 @@ struct AttnMaps {
     CUtensorMap k, v, q;
 };
 
-// Units of a part, before `parts` is looked at: from the whole batch's work, which every warp that asks adds up.  TILES:
-// for the sequences of the tile kernel, else for those of the kernel for few rows.  With t row tiles in all, cutting to
-// work / (blocks - t) units leaves no more than `blocks` parts, whatever the lengths; cutting to work / (cuts t) units, no
-// more than (cuts + 1) t.
+// What a sequence adds to the work of its kernel (TILES: the tile kernel, else the one for few rows).  One with too many rows has
+// one tile and no keys, as in work_of: the host has sized the grid for no more.
+struct Share {
+    unsigned units, tiles;
+};
+template <bool TILES>
+__device__ __forceinline__ Share share_of(const AttnParams& p, int tile, int seq) {
+    const Sequence s = sequence_at(p.batch, seq);
+    const int64_t total = (int64_t)s.rows * p.group;
+    if (total == 0 || (total > p.few_rows) != TILES) return Share{0, 0};
+    if (s.rows > p.batch.max_rows) return Share{0, 1};
+    return Share{(unsigned)(min(max(p.batch.seq_lens[seq], 0), capacity(p.batch, p.cache)) + kSplitKeys - 1) / kSplitKeys,
+                 (unsigned)min((total + tile - 1) / tile, (int64_t)1 << 20)};
+}
+
+// Units of a part, before `parts` is looked at: from the whole batch's work, which every warp that asks adds up.  With t
+// row tiles in all, cutting to work / (blocks - t) units leaves no more than `blocks` parts, whatever the lengths; cutting to
+// work / (cuts t) units, no more than (cuts + 1) t.
 template <bool TILES>
 __device__ __forceinline__ int even_units(const AttnParams& p, SplitRule rule, int tile) {
     if (rule.parts == 1) return 0;
-    const int lane = threadIdx.x & 31, room = capacity(p.batch, p.cache), kv_heads = p.heads / p.group;
+    const int lane = threadIdx.x & 31, kv_heads = p.heads / p.group;
     unsigned long long sum = 0;
     unsigned tiles = 0;
     for (int i = lane; i < p.batch.num_seqs; i += 32) {
-        const Sequence s = sequence_at(p.batch, i);
-        const int tokens = p.batch.seq_lens[i];
-        if (s.rows == 0 || ((int64_t)s.rows * p.group > p.few_rows) != TILES) continue;
-        const unsigned units = (unsigned)(min(max(tokens, 0), room) + kSplitKeys - 1) / kSplitKeys;
-        const unsigned n = (unsigned)min(((int64_t)s.rows * p.group + tile - 1) / tile, (int64_t)1 << 20);
-        sum += units * (unsigned long long)n;
-        tiles += n;
+        const Share w = share_of<TILES>(p, tile, i);
+        sum += w.units * (unsigned long long)w.tiles;
+        tiles += w.tiles;
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
@@ -93,16 +103,9 @@ __device__ __forceinline__ int tile_units(const AttnParams& p, SplitRule rule, i
     if (rule.parts == 1) return 0;
     const int lane = threadIdx.x & 31, n = p.batch.num_seqs;
     if (n > 32) return even_units<true>(p, rule, tile);
-    unsigned units = 0;                                    // of this lane's sequence
-    float count = 0.f;                                     // its row tiles, of all KV heads
-    if (lane < n) {
-        const Sequence s = sequence_at(p.batch, lane);
-        const int64_t total = (int64_t)s.rows * p.group;
-        if (s.rows > 0 && total > p.few_rows) {
-            units = (unsigned)(min(max(p.batch.seq_lens[lane], 0), capacity(p.batch, p.cache)) + kSplitKeys - 1) / kSplitKeys;
-            count = (float)((total + tile - 1) / tile * (p.heads / p.group));
-        }
-    }
+    const Share mine = lane < n ? share_of<true>(p, tile, lane) : Share{0, 0};
+    const unsigned units = mine.units;
+    const float count = (float)mine.tiles * (p.heads / p.group);          // row tiles of all KV heads
     float work = units * count, tiles = count;
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
