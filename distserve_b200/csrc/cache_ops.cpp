@@ -87,8 +87,11 @@ kvmig_pool_shape pools_of(const at::Tensor& k, const at::Tensor& v, const at::Te
     return kvmig_pool_shape{k.size(0), k.size(1), k.size(2), k.size(3), k.size(4), static_cast<int64_t>(k.element_size())};
 }
 
-// The operators compute no gradients: a call that autograd would have to follow is refused rather than cut off silently.
+// The operators compute no gradients: a call that autograd would have to follow, backward or forward, is refused rather than cut
+// off silently.
 void check_no_grad(std::initializer_list<const at::Tensor*> inputs, const char* op) {
+    for (const at::Tensor* t : inputs)
+        TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, " has no gradient, and an argument carries a forward-mode tangent");
     if (!at::GradMode::is_enabled()) return;
     for (const at::Tensor* t : inputs) TORCH_CHECK(!t->requires_grad(), op, " has no gradient: call it under torch.no_grad()");
 }
