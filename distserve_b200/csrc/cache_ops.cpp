@@ -102,6 +102,12 @@ void check_written(const at::Tensor& t, std::initializer_list<const at::Tensor*>
         if (t.numel() && o->numel()) at::assert_no_overlap(t, *o);
 }
 
+// The call has been enqueued: autograd takes note that these were overwritten.  (Tensors made in inference mode keep no count.)
+void count_written(std::initializer_list<const at::Tensor*> written) {
+    for (const at::Tensor* t : written)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // kv_cache_ops::write
 void write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, int64_t layer,
            const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& starts) {
@@ -117,6 +123,7 @@ void write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, 
     check(kvmig_cache_write(&kr, &vr, dtype, k_cache.data_ptr(), v_cache.data_ptr(), &s, layer, &b,
                             c10::cuda::getCurrentCUDAStream(k.device().index()).stream()),
           "write");
+    count_written({&k_cache, &v_cache});
 }
 
 // kv_cache_ops::read
@@ -134,6 +141,7 @@ void read(const at::Tensor& k_cache, const at::Tensor& v_cache, int64_t layer, c
     check(kvmig_cache_read(k_cache.data_ptr(), v_cache.data_ptr(), &s, layer, &b, &kr, &vr, dtype,
                            c10::cuda::getCurrentCUDAStream(k_out.device().index()).stream()),
           "read");
+    count_written({&k_out, &v_out});
 }
 
 // kv_attention_ops::paged
@@ -155,6 +163,7 @@ void paged(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_c
                                 bytes > 0 ? workspace.data_ptr() : nullptr, bytes,
                                 c10::cuda::getCurrentCUDAStream(q.device().index()).stream()),
           "paged");
+    count_written({&out});
 }
 
 // kv_attention_ops::prompt
@@ -172,6 +181,7 @@ void prompt(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const
     check(kvmig_prompt_attention(&qr, &kr, &vr, &orow, dtype, q.size(2), &b, scale,
                                  c10::cuda::getCurrentCUDAStream(q.device().index()).stream()),
           "prompt");
+    count_written({&out});
 }
 
 }  // namespace
