@@ -1,4 +1,5 @@
-"""What the cache and attention operators refuse before they look for a device: calls that autograd would have to follow."""
+"""What the cache and attention operators refuse before they look for a device: calls that autograd would have to follow, and
+workspaces that do not fit."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -47,3 +48,27 @@ def test_leaves_that_require_a_gradient_are_refused():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):       # then only the device is missing
             call()
+
+
+@pytest.mark.parametrize("elem_size", [1, 2])
+@pytest.mark.parametrize("num_seqs,max_rows", [(1, 1), (3, 4), (2, 300)])
+def test_a_workspace_that_does_not_fit_is_refused(built_libs, num_seqs, max_rows, elem_size):
+    """Partial results go there, so it is what keeps them in bounds: too small, absent or misaligned never reaches a launch."""
+    from distserve_b200 import capi
+
+    shape = capi.PoolShape.of(num_blocks=4096, num_layers=2, num_heads=2, block_size=16, head_dim=64 + (4 if elem_size == 1 else 0), elem_size=elem_size)
+    rows = capi.Rows(0x1000, 8, 512, 64)
+    batch = capi.Batch(num_seqs, num_seqs * max_rows, max_rows, 0x9000, 0xA000, 0xB000, 1024, 1024)
+    need = capi.paged_attention_workspace(shape, 8, batch)
+    assert need > 0 and need == capi.paged_attention_workspace(shape, 8, batch)
+
+    def call(workspace, size):
+        capi.paged_attention(rows, rows, 0, 0x100000, 0x200000, shape, 1, batch, 0.125, workspace, size)
+
+    for workspace, size in ((0x40000, need - 1), (0x40000, 0), (0x40000, -1), (0, need), (0x40008, need), (0x40001, 2 * need)):
+        with pytest.raises(capi.KvmigError, match=f"needs a workspace of {need} bytes") as e:
+            call(workspace, size)
+        assert e.value.code == capi.EINVAL
+    if not torch.cuda.is_available():
+        with pytest.raises(capi.KvmigError, match="cudaGetDevice"):         # enough of it: then only the device is missing
+            call(0x40000, need)
