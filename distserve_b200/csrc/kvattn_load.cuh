@@ -19,9 +19,8 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int j) {
     return (uint32_t)((j >> 3) * (kTileKeys * 128) + r * 128 + (((j & 7) ^ (r & 7)) << 4));
 }
 
-// SCALED: values are widened as kvmig_cache_read gives them, in the rows' type.  Otherwise to the codes' own values in
-// fp16, and the tile's scales go into `scales`, [slot][128].
-template <int HD, bool BF16, bool PAGED, bool E4M3, int WARPS, int SLOTS, int RAW_SLOTS, bool SCALED>
+// Codes are widened as kvmig_cache_read gives them, in the rows' type.
+template <int HD, bool BF16, bool PAGED, bool E4M3, int WARPS, int SLOTS, int RAW_SLOTS>
 struct TileLoader {
     static constexpr int kSlot = kTileKeys * HD * 2, kRawSlot = kTileKeys * (HD + 4);
     static constexpr int kPieces = HD / 8, kRowsAtOnce = 32 / kPieces;        // of a 16-bit row; rows that a warp copies at once
@@ -35,7 +34,6 @@ struct TileLoader {
     unsigned char *const ring, *const raw;
     const uint32_t full, empty, raw_full, raw_empty, tail;
     volatile int* const flags;
-    float* scales = nullptr;
     bool bad = false, ok = true;             // a block that is not there; no wait has run out
     int issued = 0;                          // tiles that the copy engine was given
 
@@ -248,13 +246,7 @@ struct TileLoader {
                 const int g = w + x * WARPS, r = g * kRawRows + lane / kRowPieces, j = lane % kRowPieces;
                 if (g >= kTileKeys / kRawRows) break;
                 uint4 lo, hi;
-                if (SCALED) {
-                    widen16<BF16>(codes[x], scale[x], lo, hi);
-                } else {
-                    lo = make_uint4(widen2(codes[x].x), widen2(codes[x].x >> 16), widen2(codes[x].y), widen2(codes[x].y >> 16));
-                    hi = make_uint4(widen2(codes[x].z), widen2(codes[x].z >> 16), widen2(codes[x].w), widen2(codes[x].w >> 16));
-                    if (j == 0) scales[slot * kTileKeys + r] = scale[x];
-                }
+                widen16<BF16>(codes[x], scale[x], lo, hi);
                 if (c % 2 && r >= keys) lo = hi = make_uint4(0, 0, 0, 0);
                 const bool second = j >= kRowPieces / 2;                  // half of the lanes store their second piece first: other banks
                 *reinterpret_cast<uint4*>(to + tile_offset(r, 2 * j + second)) = second ? hi : lo;

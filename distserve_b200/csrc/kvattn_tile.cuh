@@ -311,9 +311,9 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
             }
         }
         copy_commit();
-        TileLoader<HD, BF16, PAGED, E4M3, kLoadWarps, T::kSlots, T::kRawSlots, true> loader(p, maps, w, seq, kv_head, s.first, range.begin, range.end,
-                                                                                         smem + T::kRing, smem + T::kRaw, full(0), empty(0), raw_full,
-                                                                                         raw_empty, tail, flags);
+        TileLoader<HD, BF16, PAGED, E4M3, kLoadWarps, T::kSlots, T::kRawSlots> loader(p, maps, w, seq, kv_head, s.first, range.begin, range.end,
+                                                                                   smem + T::kRing, smem + T::kRaw, full(0), empty(0), raw_full,
+                                                                                   raw_empty, tail, flags);
         loader.run(2 * steps, [&] {
             if (lane == 0 && !(q_by_engine && w == 0)) barrier_arrive(q_full);
         });
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__((TileShape<HD, E4M3>::kThreads), 1) attend_til
     } else {
         // ---- products: one lane issues them all -----------------------------------------------------------
         if (steps > 0) {
-            const uint32_t s_kind = product_kind(BF16, kTileRows, kTileKeys, false, false) | (p.scale_log2 < 0.f ? 1u << 13 : 0u);
+            const uint32_t s_kind = product_kind(BF16, kTileRows, kTileKeys, false, p.scale_log2 < 0.f);
             constexpr uint32_t o_kind = product_kind(BF16, kTileRows, HD, true, false);
             const bool leader = elect_one();
             const uint64_t q_desc = operand(base, 16, 1024), k_desc = operand(base + T::kRing, 16, 1024),

@@ -79,8 +79,6 @@ __host__ __device__ __forceinline__ int capacity(const BatchView& b, const Cache
 
 template <bool BF16> struct Half;
 template <> struct Half<false> {
-    using T = __half;
-    using T2 = __half2;
     static constexpr uint32_t kInf = 0x7c00, kNan2 = 0x7fff7fff;
     static __device__ __forceinline__ float2 to_float2(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
     static __device__ __forceinline__ uint32_t from_float2(float a, float b) {
@@ -90,8 +88,6 @@ template <> struct Half<false> {
     static __device__ __forceinline__ float largest() { return 65504.f; }
 };
 template <> struct Half<true> {
-    using T = __nv_bfloat16;
-    using T2 = __nv_bfloat162;
     static constexpr uint32_t kInf = 0x7f80, kNan2 = 0x7fff7fff;
     static __device__ __forceinline__ float2 to_float2(uint32_t w) {
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));

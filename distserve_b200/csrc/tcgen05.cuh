@@ -122,10 +122,6 @@ __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&x)[32])
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
         "%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at), KVMIG_W8(x, 0), KVMIG_W8(x, 8), KVMIG_W8(x, 16), KVMIG_W8(x, 24) : "memory");
 }
-__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&x)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 ::"r"(at), KVMIG_W8(x, 0), KVMIG_W8(x, 8) : "memory");
-}
 #undef KVMIG_R8
 #undef KVMIG_X8
 #undef KVMIG_W8
