@@ -51,6 +51,8 @@ class CacheConfig:
                  gpu_memory_utilization: float = 0.9, cpu_swap_space: int = 0, kv_format: str = "model") -> None:
         if kv_format not in ("model", "e4m3"):
             raise ValueError(f"kv_format must be 'model' or 'e4m3', not {kv_format!r}")
+        if kv_format == "e4m3" and block_size % 4:
+            raise ValueError(f"blocks of an e4m3 pool hold a multiple of 4 tokens, not {block_size}")
         self.kv_format = kv_format
         self.block_size = block_size
         self.max_num_blocks_per_req = max_num_blocks_per_req
@@ -85,6 +87,13 @@ class KVModelConfig:
 
     def get_head_size(self) -> int:
         return self.head_dim
+
+    def check_kv_format(self, kv_format: str) -> None:
+        """Raises unless pools of this format can be written and read for this model (float32 pools of the model's own
+        type can be moved and swapped, which is all that the operators on their contents leave to them)."""
+        if kv_format == "e4m3" and (self.get_dtype_size() != 2 or self.head_dim % 16 or not 0 < self.head_dim <= 256):
+            raise ValueError(f"e4m3 pools hold rows of float16 or bfloat16 with a head_dim that is a multiple of 16 up to 256, not of "
+                             f"{self.dtype} with {self.head_dim}")
 
     def get_dtype_size(self) -> int:
         return {"float16": 2, "bfloat16": 2, "float32": 4}[self.dtype]

@@ -52,6 +52,8 @@ class _SwapMark:
 class KVWorker:
     def __init__(self, worker_id: int, stage, model_config: KVModelConfig, cache_config: CacheConfig,
                  parallel_config: ParallelConfig = ParallelConfig(), device: Optional[int] = None) -> None:
+        if getattr(cache_config, "kv_format", "model") != "model":
+            model_config.check_kv_format(cache_config.kv_format)
         if not torch.cuda.is_available():
             raise RuntimeError("KVWorker needs a CUDA device; there is no CPU implementation of this path")
         load_ops()
