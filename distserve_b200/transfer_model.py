@@ -9,7 +9,8 @@ time = fixed cost per call + bytes into the slowest decoding worker / bandwidth
 
 * Each decoding worker pulls its own rectangle concurrently, so the request's
   transfer time is that of ONE worker's share: ``2·(L/dec_pp)·(H/dec_tp)·
-  block_size·head_dim·elem`` bytes per block.
+  block_size·head_dim·elem`` bytes per block, or ``·(head_dim + 4)`` where
+  ``kv_format`` is "e4m3".
 * Across NVLink a call moves 790 GB/s into a GPU once it is running, plus about
   14 µs of ramp-up and tail; an awaited call adds the platform's
   launch-and-wait round trip, about 15 µs more.  Calls enqueued back to back
@@ -39,25 +40,25 @@ def blocks_for(prompt_len: int, block_size: int) -> int:
     return -(-prompt_len // block_size)
 
 
-def bytes_per_block_per_worker(model: KVModelConfig, dec: ParallelConfig, block_size: int) -> int:
-    return 2 * model.block_bytes(dec, block_size)
+def bytes_per_block_per_worker(model: KVModelConfig, dec: ParallelConfig, block_size: int, kv_format: str = "model") -> int:
+    return 2 * model.block_bytes(dec, block_size, kv_format)
 
 
 def migration_seconds(prompt_len: int, model: KVModelConfig, dec: ParallelConfig, block_size: int = 16,
-                      link: LinkModel = NVLINK5, awaited: bool = True) -> float:
+                      link: LinkModel = NVLINK5, awaited: bool = True, kv_format: str = "model") -> float:
     """Time until the request's KV is in place on every decoding worker."""
     if prompt_len <= 0:
         return 0.0
-    payload = blocks_for(prompt_len, block_size) * bytes_per_block_per_worker(model, dec, block_size)
+    payload = blocks_for(prompt_len, block_size) * bytes_per_block_per_worker(model, dec, block_size, kv_format)
     fixed_us = link.awaited_call_us if awaited else link.chained_call_us
     return fixed_us * 1e-6 + payload / (link.payload_GBps * 1e9)
 
 
 def effective_GBps(prompt_len: int, model: KVModelConfig, dec: ParallelConfig, block_size: int = 16,
-                   link: LinkModel = NVLINK5, awaited: bool = True) -> float:
+                   link: LinkModel = NVLINK5, awaited: bool = True, kv_format: str = "model") -> float:
     """Payload bytes per second into one decoding worker for requests of this length."""
-    payload = blocks_for(prompt_len, block_size) * bytes_per_block_per_worker(model, dec, block_size)
-    return payload / migration_seconds(prompt_len, model, dec, block_size, link, awaited) / 1e9
+    payload = blocks_for(prompt_len, block_size) * bytes_per_block_per_worker(model, dec, block_size, kv_format)
+    return payload / migration_seconds(prompt_len, model, dec, block_size, link, awaited, kv_format) / 1e9
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -71,7 +72,7 @@ CROSS_NODE_400G = LinkModel(payload_GBps=45.0, awaited_call_us=60.0, chained_cal
 
 
 def exit_prefill_delay_ms(prompt_len: int, model: KVModelConfig, dec: ParallelConfig, block_size: int = 16,
-                          link: LinkModel = NVLINK5, streamed_groups: int = 0) -> float:
+                          link: LinkModel = NVLINK5, streamed_groups: int = 0, kv_format: str = "model") -> float:
     """Delay to charge between the end of a request's prefill and its entry into the decoding stage, in the
     simulator's time unit (milliseconds): what a hook in ``Worker._exit_prefill`` would wait before it calls
     ``forward_decode`` (simdistserve/base/worker.py:264-279 hands the request over with no delay at all).
@@ -80,7 +81,7 @@ def exit_prefill_delay_ms(prompt_len: int, model: KVModelConfig, dec: ParallelCo
     only the last group's share of the payload is left after prefill ends."""
     if prompt_len <= 0:
         return 0.0
-    payload = blocks_for(prompt_len, block_size) * bytes_per_block_per_worker(model, dec, block_size)
+    payload = blocks_for(prompt_len, block_size) * bytes_per_block_per_worker(model, dec, block_size, kv_format)
     if streamed_groups > 0:
         payload = payload / streamed_groups
     return (link.awaited_call_us * 1e-6 + payload / (link.payload_GBps * 1e9)) * 1e3
@@ -101,7 +102,8 @@ class DecodePlacement:
 
 
 def pick_decode_placement(candidates, prompt_lens, model: KVModelConfig, max_handoff_ms: float, block_size: int = 16,
-                          charge_transfer: bool = True, streamed_groups: int = 0, percentile: float = 0.9):
+                          charge_transfer: bool = True, streamed_groups: int = 0, percentile: float = 0.9,
+                          kv_format: str = "model"):
     """The candidate with the highest goodput per GPU among those whose hand-off delay (at the given percentile of
     the prompt lengths) fits `max_handoff_ms`.  With ``charge_transfer`` off every candidate fits — the reference
     simulator's view, in which the transfer is free.  Returns (candidate, its hand-off delay in ms); raises if
@@ -110,7 +112,7 @@ def pick_decode_placement(candidates, prompt_lens, model: KVModelConfig, max_han
     at = lens[min(len(lens) - 1, int(percentile * len(lens)))]
     best = None
     for c in candidates:
-        delay = exit_prefill_delay_ms(at, model, c.worker(), block_size, c.link, streamed_groups) if charge_transfer else 0.0
+        delay = exit_prefill_delay_ms(at, model, c.worker(), block_size, c.link, streamed_groups, kv_format) if charge_transfer else 0.0
         if delay <= max_handoff_ms and (best is None or c.goodput_per_gpu > best[0].goodput_per_gpu):
             best = (c, delay)
     if best is None:
