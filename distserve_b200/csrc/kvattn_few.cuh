@@ -269,8 +269,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
                     inverse[n][e] = scale == 0.f ? 0.f : __fdividef(kSumUnit, scale);              // 0: a key that is not there
                 }
         };
-        // With 16 rows early enough not to be waited for (32 x 2000 tokens: 3% faster); 32 have no registers to keep it in (4% slower).
-        if (E4M3 && MT == 1) find_inverse();
+        if (E4M3) find_inverse();
         const bool all = first_key(i) + kFewKeys <= seen_by_all;               // every row sees all of these keys
         float top[MT][2];
         auto find_top = [&] {
@@ -299,8 +298,9 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
         bool grown = false;
 #pragma unroll
         for (int x = 0; x < MT; ++x) grown |= top[x][0] > m[x][0] || top[x][1] > m[x][1];
+        auto is_one = [](float log2_scale) { return fabsf(log2_scale) < 0.5f; };        // log2 is approximate, scales are powers of two
         if (__any_sync(0xffffffffu, grown)) {
-            if (E4M3 && __any_sync(0xffffffffu, scales[kFewKeys + (lane & 15)] == 1.f)) {
+            if (E4M3 && __any_sync(0xffffffffu, is_one(lift[0][0]) || is_one(lift[0][1]) || is_one(lift[1][0]) || is_one(lift[1][1]))) {
                 // Whose rows of V are zeros?  A lane looks at half of key (lane & 15)'s.
                 uint32_t codes = 0;
 #pragma unroll 1
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
                             }
                         }
                 find_top();
-                if (MT == 1) find_inverse();
+                find_inverse();
             }
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
@@ -341,7 +341,6 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) attend_few(const __grid
                     for (int e = 0; e < 4; ++e) o[x][n][e] *= keep[e / 2];
             }
         }
-        if (E4M3 && MT > 1) find_inverse();
         uint32_t a[MT][4];
 #pragma unroll
         for (int x = 0; x < MT; ++x) {
