@@ -15,9 +15,13 @@
 //     lower end fp16 holds P_j to eleven bits down to 2^-29 of its largest value and to 2^-40 of it below.  A row's scale is the
 //     size of its values, so that is what a value weighs in the output, but for a row of zeros, whose scale is 1 whatever
 //     its neighbours' are: one that would raise m counts with kZeroRowScale instead, or it would push the others out of the range.
-// Measured: 64 requests with 40 heads of 128, 41k cached tokens, 838 MB: 138 us (6.1 TB/s, 95% of a copy); 32 requests of
-// 2000 tokens, 16 heads: 83 us from 16 bits (6.3 TB/s), 74 us from e4m3 (3.7 TB/s: instructions per byte, a third of them
-// widening, are what bounds it; a third block per SM with a smaller ring gained nothing).
+// Measured: 64 requests with 40 heads of 128, 41k cached tokens, 838 MB: 137 us (6.1 TB/s, 95% of a copy); 32 requests of
+// 2000 tokens, 16 heads: 85 us from 16 bits (6.1 TB/s), 76 us from e4m3 (3.6 TB/s).  From e4m3 it is latency that bounds it: DRAM
+// is 43% busy and 0.43 of the issue slots are used, by two warps to a scheduler that each go through a chain of copies, widening,
+// products, maximum, exponentials and products for 16 keys (4.1 cycles from one instruction of a warp to its next, 1.3 of them
+// for the result of the one before, 0.8 for copies).  A third block per SM with a smaller ring gained nothing.
+// The look for rows of zeros costs what its instructions take to fetch: 0.5 us of 10 for 16 requests of 300 tokens, nothing
+// that shows for longer ones.
 #pragma once
 
 #include "kvattn_device.cuh"
@@ -27,7 +31,7 @@ namespace kvmig {
 constexpr int kFewKeys = 16;
 // Rows of a sequence and KV head up to which this kernel is used.  Beyond 32 it reads the cache twice, which the tile kernel
 // beats on 16-bit pools (8 sequences of 4000 tokens, 16 KV heads: 32 rows 73 us here and 76 there, 48 rows 109 and 77) but not
-// where it has to widen codes for tiles of 256 rows (64 rows 122 and 147, 96 rows 204 and 146).
+// where it has to widen codes for tiles of 256 rows (64 rows 116 and 147, 96 rows 204 and 146).
 constexpr int few_most(bool e4m3) { return e4m3 ? 64 : 32; }
 
 // Quantised pools: P_j's largest value is 2^15 (kTopLog2).  The sum counts P_j 2^-6 / s_j (kSumUnit), since 1 / s_j alone reaches

@@ -13,7 +13,8 @@
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time; until then P may be as large
 // as 256, which costs no precision.  Tensor memory: S0 S1 O0 O1, 128 columns each.
 //
-// Measured: one prompt of 4096 tokens, 32/4 heads of 128: 130-137 us, 1.0-1.06 PFLOP/s, 0.6 of the library's best rate.
+// Measured: one prompt of 4096 tokens, 32/4 heads of 128: 137 us in bf16, 1.0 PFLOP/s, 0.6 of the library's best rate; 155 us in
+// fp16, 0.89 PFLOP/s.
 // A step of 256 rows by 128 keys takes 3100 cycles where its products need 2048: each tile waits for its own chain of
 // scores (512 cycles and a wake-up), softmax (2000, of which the special function unit needs 1024) and products.  Tried
 // and slower: a quarter or half of the exponentials as polynomials (2%, 8%), two softmax threads per row (50%), a warp for
@@ -33,6 +34,7 @@ template <int HD, bool E4M3> struct TileShape {
     static constexpr int kSlots = E4M3 ? 3 : 5;
     static constexpr int kLoadWarps = E4M3 ? 7 : 3, kThreads = kSoftmaxThreads + kLoadWarps * 32 + 32;
     // Registers of a softmax thread and of the others: together what the block is launched with (168 or 128 a thread).
+    // Over quantised pools 196 bytes a thread are spilled and 216 reloaded (76 and 88 at a head_dim of 64).
     static constexpr int kSoftmaxRegisters = E4M3 ? 200 : 208, kOtherRegisters = E4M3 ? 56 : 88;
     static constexpr int kRawSlot = E4M3 ? kTileKeys * (HD + 4) : 0;        // codes, then scales
     static constexpr int kRawSlots = E4M3 ? 3 : 0;
