@@ -20,8 +20,9 @@
 // is 43% busy and 0.43 of the issue slots are used, by two warps to a scheduler that each go through a chain of copies, widening,
 // products, maximum, exponentials and products for 16 keys (4.1 cycles from one instruction of a warp to its next, 1.3 of them
 // for the result of the one before, 0.8 for copies).  A third block per SM with a smaller ring gained nothing.
-// The look for rows of zeros costs what its instructions take to fetch: 0.5 us of 10 for 16 requests of 300 tokens, nothing
-// that shows for longer ones.
+// Rows of zeros cost short sequences something, since their maxima still grow: 16 requests of 300 tokens, 12 heads of 64, 9.4 us
+// without the look for them and the shift by 2^15, 10.2 with; 64 of 640, 40 heads, 127 and 129; 32 of 2000 as before.  A vote per
+// group of 16 keys ahead of the scores took 2-4% of all of them, the same code as a function or a second turn 2-5% of 32 rows.
 #pragma once
 
 #include "kvattn_device.cuh"
